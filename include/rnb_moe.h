@@ -347,6 +347,157 @@ RNB_API int rnb_moe_block_norm_fwd(const rnb_moe_desc* d, rnb_ep* ep, const void
 RNB_API int rnb_stage_timing(int enable);
 RNB_API int rnb_stage_times(float* ms, int max_stages, int* calls);
 
+/* ---- Attention over a paged key-value cache (serving; no reference
+ * counterpart: the reference leaves attention to mlx-lm) ----
+ * The other half of a full-attention decoder layer around the block above, in
+ * the order of a serving step: rnb_kv_plan gives the step's new tokens their
+ * pages, slots and positions; rnb_rope_append norms and rotates the queries
+ * and keys and writes keys and values to the cache; rnb_paged_attention reads
+ * it.  All three take lengths, tables and positions from device memory, so a
+ * step captured in a CUDA graph replays with other lengths.
+ *
+ * The cache of a layer is two tensors of pages, [num_pages][n_kv_heads]
+ * [page_size][head_dim], in bf16 or fp16; page and head strides are free
+ * (multiples of 8 elements), a head's page is contiguous.  Position p of a
+ * request lives in row p % page_size of page table[p / page_size]; a slot is
+ * page * page_size + row.  page_size: 16, 32, 64, 128 or 256; head_dim: 64,
+ * 128 or 256; at most 2^31 - 1 slots.
+ *
+ * What a device-side length, slot or page id asks for beyond the tensors is
+ * left out, never read or written, and sets a bit in a status word that the
+ * library keeps for each device; rnb_kv_status reads and clears it. */
+#define RNB_STATUS_NO_PAGES 0x4u /* a plan was void: too few pages, table columns or token rows */
+
+#define RNB_DTYPE_BF16 0
+#define RNB_DTYPE_F16 1
+
+typedef struct rnb_kv_cache {
+  int32_t dtype;      /* RNB_DTYPE_* */
+  int32_t num_pages;
+  int32_t page_size;
+  int32_t n_kv_heads;
+  int32_t head_dim;
+  int32_t reserved0;
+  void* k;
+  void* v;
+  int64_t k_page_stride; /* strides in elements */
+  int64_t k_head_stride;
+  int64_t v_page_stride;
+  int64_t v_head_stride;
+} rnb_kv_cache;
+
+/* Pages, slots and positions of one step.  Request b holds ctx_lens[b] cached
+ * tokens in the first ceil(ctx / page_size) entries of its table row and gets
+ * new_lens[b] more (0: idle).  The pages it lacks are taken from the end of
+ * the free list free_pages[0 .. *free_count), requests in order; their ids go
+ * into the table (other entries are left as they were) and
+ *   seq_lens  [B]    ctx + new (may not be ctx_lens or new_lens itself)
+ *   cu_q      [B+1]  first new-token row of each request, then their number
+ *   positions [max_tokens], slots [max_tokens]  of every new-token row; rows
+ *             behind the last request get position 0 and slot -1
+ *   free_count_out [1]  pages left (may not be free_count itself)
+ * All or nothing: if the pages, the table's columns, max_tokens or 31 bits do
+ * not suffice, or a length is negative, nothing is taken, seq_lens = ctx_lens,
+ * cu_q = 0, every slot is -1 and RNB_STATUS_NO_PAGES is set, so the step's
+ * later calls do nothing.  A call with the same inputs gives the same outputs
+ * again.  B <= 16384.  A page id outside [0, num_pages) gives slot -1 and
+ * RNB_STATUS_BAD_INDEX. */
+RNB_API int rnb_kv_plan(int B, int table_cols, int page_size, int num_pages, int max_tokens, int32_t* table,
+                        const int32_t* ctx_lens, const int32_t* new_lens, const int32_t* free_pages,
+                        int free_capacity, const int32_t* free_count, int32_t* seq_lens, int32_t* cu_q,
+                        int32_t* positions, int32_t* slots, int32_t* free_count_out, void* stream);
+/* Gives the pages of finished requests back: for every b with finished[b] != 0
+ * the first ceil(lens[b] / page_size) entries of its table row are appended to
+ * free_pages behind *free_count, requests in order, and lens_out[b] = 0 (else
+ * lens[b]; lens_out may be lens).  free_count_out as in rnb_kv_plan.  If they
+ * do not fit free_capacity, or a length is negative or beyond the table, the
+ * call does nothing (lens_out = lens) and sets RNB_STATUS_NO_PAGES.  One CTA:
+ * B <= 16384. */
+RNB_API int rnb_kv_release(int B, int table_cols, int page_size, const int32_t* table, const int32_t* lens,
+                           const int32_t* finished, int32_t* free_pages, int free_capacity,
+                           const int32_t* free_count, int32_t* lens_out, int32_t* free_count_out, void* stream);
+/* Status bits (RNB_STATUS_*) of the attention-side calls on the current
+ * device since the last read: copies them to *status and clears them.
+ * Synchronises the stream; not for use while a stream is being captured. */
+RNB_API int rnb_kv_status(uint32_t* status, void* stream);
+
+/* Rotary positions with one to four axes, after an optional RMSNorm of each
+ * head, and the append to the cache.  For every token t, head h and pair
+ * i < rot/2 of a query or key row x (normed: x * rsqrt(mean x^2 + eps) * w):
+ *   angle = positions[axis(i)][t] * inv_freq[i]          (64-bit product)
+ *   x'[i]         = x[i] cos(angle) - x[i + rot/2] sin(angle)
+ *   x'[i + rot/2] = x[i + rot/2] cos(angle) + x[i] sin(angle)
+ * elements from rot on pass through; fp32 throughout, rounded once.  With
+ * n_axes axes, sections[a] of the rot/2 frequencies belong to axis a: one
+ * section after the other (interleaved 0), or in turns (interleaved 1: axis
+ * a >= 1 has i = a, a + n_axes, ..., sections[a] of them; axis 0 the rest).
+ * Queries go to q_out [T][n_q_heads][head_dim] (may be q itself if q is
+ * packed like that); rotated keys and values (as they are) go to the cache
+ * row of slots[t].  A row with slots[t] < 0 is left alone altogether; with a
+ * slot beyond the cache only its query is written, and RNB_STATUS_BAD_INDEX
+ * is set.  Two rows of one call with the same slot leave either's values.
+ * cache, k, v and slots may be NULL together: then only the queries are
+ * turned.  rot: a multiple of 16, at most head_dim. */
+typedef struct rnb_rope_desc {
+  int32_t dtype;      /* RNB_DTYPE_* of q, k, v, the cache and the norm weights */
+  int32_t T;
+  int32_t n_q_heads;
+  int32_t n_kv_heads; /* 0 without a cache */
+  int32_t head_dim;
+  int32_t rot;
+  int32_t n_axes;
+  int32_t interleaved;
+  int32_t sections[4];
+  float eps;
+  int32_t reserved0;
+  int64_t q_token_stride; /* strides in elements, multiples of 8 */
+  int64_t q_head_stride;
+  int64_t k_token_stride;
+  int64_t k_head_stride;
+  int64_t v_token_stride;
+  int64_t v_head_stride;
+} rnb_rope_desc;
+RNB_API int rnb_rope_append(const rnb_rope_desc* d, const void* q, const void* k, const void* v, const void* q_norm_w,
+                            const void* k_norm_w, const int32_t* positions, const float* inv_freq,
+                            const int32_t* slots, const rnb_kv_cache* cache, void* q_out, void* stream);
+
+/* Causal attention of the step's query rows over the paged cache.  Request b
+ * has the query rows [cu_q[b], cu_q[b+1]) (cu_q NULL: row b alone, T == B),
+ * the last of its seq_lens[b] positions; row i at position
+ * p = seq_len - rows + i sees the positions j <= p, and j > p - window when
+ * window > 0.  Query head h reads key head h / (n_q_heads / n_kv_heads):
+ *   out[t][h] = softmax_j(scale * q . k_j) v_j
+ * times sigmoid(gate[t][h]) elementwise when gate is given, rounded once;
+ * lse[t][h] (optional, fp32) = log sum_j exp(scale * q . k_j).  A row that
+ * sees nothing gives zeros and -inf.  Rows behind cu_q[B] are left as they
+ * were.  Softmax statistics and sums are fp32; probabilities are rounded to
+ * the cache's type for the product with V.  What lies in the cache behind a
+ * request's length never counts, whatever its bits; within the length values
+ * must be finite, except that a request's single row may have any bits in
+ * positions that its window leaves out.  Any number of rows per request;
+ * requests in any mix.  max_q (0: unknown) bounds the rows of a request and
+ * only picks the kernels.  The workspace needs no initial state; calls that
+ * may overlap need one each.  Results do not depend on timing: equal inputs
+ * give equal bits. */
+typedef struct rnb_attn_desc {
+  int32_t B;
+  int32_t T;          /* rows of q and out */
+  int32_t n_q_heads;
+  int32_t table_cols;
+  int32_t max_q;
+  int32_t window;
+  float scale;
+  int32_t reserved0;
+  int64_t q_token_stride; /* strides in elements, multiples of 8 */
+  int64_t q_head_stride;
+  int64_t gate_token_stride;
+  int64_t gate_head_stride;
+} rnb_attn_desc;
+RNB_API int rnb_paged_attention_workspace_size(const rnb_attn_desc* d, const rnb_kv_cache* cache, size_t* bytes);
+RNB_API int rnb_paged_attention(const rnb_attn_desc* d, const rnb_kv_cache* cache, const void* q, const void* gate,
+                                const int32_t* table, const int32_t* seq_lens, const int32_t* cu_q, void* out,
+                                float* lse, void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

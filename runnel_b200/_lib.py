@@ -26,6 +26,7 @@ ERRORS = {
 }
 STATUS_BAD_INDEX = 0x1
 STATUS_TIMEOUT = 0x2
+STATUS_NO_PAGES = 0x4
 FLAG_SHARED_ON_THIS_RANK = 0x1
 FLAG_NO_SHARED = 0x2
 FLAG_Y_F32 = 0x4
@@ -54,7 +55,41 @@ class RnbMoeDesc(ctypes.Structure):
     ]
 
 
+class RnbKvCache(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("num_pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("reserved0", ctypes.c_int32),
+        ("k", _vp), ("v", _vp),
+        ("k_page_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+        ("v_page_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64),
+    ]
+
+
+class RnbRopeDesc(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("T", ctypes.c_int32), ("n_q_heads", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("rot", ctypes.c_int32),
+        ("n_axes", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("sections", ctypes.c_int32 * 4),
+        ("eps", ctypes.c_float), ("reserved0", ctypes.c_int32),
+        ("q_token_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+        ("k_token_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+        ("v_token_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64),
+    ]
+
+
+class RnbAttnDesc(ctypes.Structure):
+    _fields_ = [
+        ("B", ctypes.c_int32), ("T", ctypes.c_int32), ("n_q_heads", ctypes.c_int32),
+        ("table_cols", ctypes.c_int32), ("max_q", ctypes.c_int32), ("window", ctypes.c_int32),
+        ("scale", ctypes.c_float), ("reserved0", ctypes.c_int32),
+        ("q_token_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+        ("gate_token_stride", ctypes.c_int64), ("gate_head_stride", ctypes.c_int64),
+    ]
+
+
 _DescP = ctypes.POINTER(RnbMoeDesc)
+_CacheP = ctypes.POINTER(RnbKvCache)
+_i = ctypes.c_int
 SIGNATURES = {
     "rnb_version": (ctypes.c_int, []),
     "rnb_last_error": (ctypes.c_char_p, []),
@@ -91,6 +126,13 @@ SIGNATURES = {
     "rnb_moe_block_norm_fwd": (ctypes.c_int, [_DescP, _vp, _vp, _vp, _vp, ctypes.c_float, _vp, _vp, _vp, _vp, _sz,
                                               _vp]),
     "rnb_add_rmsnorm": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_float, _vp]),
+    "rnb_kv_plan": (_i, [_i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "rnb_kv_release": (_i, [_i, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp]),
+    "rnb_kv_status": (_i, [ctypes.POINTER(ctypes.c_uint32), _vp]),
+    "rnb_rope_append": (_i, [ctypes.POINTER(RnbRopeDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _CacheP, _vp, _vp]),
+    "rnb_paged_attention_workspace_size": (_i, [ctypes.POINTER(RnbAttnDesc), _CacheP, ctypes.POINTER(_sz)]),
+    "rnb_paged_attention": (_i, [ctypes.POINTER(RnbAttnDesc), _CacheP, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
+                                 _vp]),
     "rnb_stage_timing": (ctypes.c_int, [ctypes.c_int]),
     "rnb_stage_times": (ctypes.c_int, [ctypes.POINTER(ctypes.c_float), ctypes.c_int, ctypes.POINTER(ctypes.c_int)]),
 }

@@ -1,0 +1,634 @@
+// rnb_attn.cu -- attention over the paged cache for few query rows a request
+// (one new token, a few drafted ones), split over the cache's length and joined
+// (rnb_paged_attention).
+//
+// For the R <= 16 query rows that share a key head (one token's group of query
+// heads, or several tokens'), with s = scale q.k and running m = max s,
+// l = sum e^(s-m), o = sum e^(s-m) v, one pass over K and V gives o/l.  Every
+// cached token is 4 D bytes for 4 R D flops: HBM bounds it, so what counts is
+// bytes in flight, an even split, and few instructions a byte.
+//
+// * Orientation.  S^T = K Q^T and O^T = V^T P^T: the 16 tokens of a subtile are
+//   the m rows of mma m16n8k16 and the query rows its 8 columns, so a group of
+//   up to 8 rows fills the instruction, and O takes D/4 registers a lane for 8
+//   rows (D/2 the other way around).
+// * No staging.  The contraction order is free, so K enters the A operand as
+//   loaded: lane (g, c) reads 16 bytes, 8 consecutive elements, of token g and
+//   of token g + 8, and the queries are read in the same order.  For V a lane
+//   reads 16 bytes of four tokens and interleaves pairs of tokens with byte
+//   permutes; which element of the head is which m row is free again.  Each
+//   load instruction covers whole 64-byte (K) or 128-byte (V) pieces of rows,
+//   shared memory holds nothing but the join of the warps, and a warp has up
+//   to 16 KB in flight.  P^T leaves the S accumulators by one 8x8 transpose
+//   (movmatrix) an operand register.
+// * Split.  A unit is 64 positions of one (request, key head, row tile).  Every
+//   CTA sums the units of all requests from the lengths on the device, takes an
+//   equal contiguous share, and so has at most two tiles that it does not
+//   cover alone; those leave (m, l, o) in the workspace, and a second kernel
+//   adds a tile's parts in order.
+#include <cuda_runtime.h>
+#include <limits.h>
+#include <stdint.h>
+
+#include <string>
+
+#include "rnb_attn.cuh"
+
+namespace rnb {
+
+__device__ uint32_t g_attn_status;
+
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kUnit = 64;  // positions
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 8x8 transpose of 16-bit elements across the warp.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void mma_t(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                      uint32_t b1);
+template <>
+__device__ __forceinline__ void mma_t<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  mma_f16(d, a0, a1, a2, a3, b0, b1);
+}
+template <>
+__device__ __forceinline__ void mma_t<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                     uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// One request's share of the work.
+struct Request {
+  int q0, rows, len;      // first query row, rows, cached positions
+  int blk0, nblk, ntile;  // first unit of positions, units, row tiles
+};
+
+template <int R>
+__device__ __forceinline__ Request request_of(const AttnArgs& a, int c0, int c1, int len) {
+  Request r;
+  r.q0 = min(max(c0, 0), a.T);
+  r.rows = min(max(c1, r.q0), a.T) - r.q0;
+  r.len = min(max(len, 0), a.max_kv);
+  const int work = r.rows * a.group < a.few_rows ? r.rows * a.group : 0;
+  r.ntile = (work + R - 1) / R;
+  const int lo = a.window > 0 ? max(0, r.len - r.rows - a.window + 1) : 0;
+  r.blk0 = lo / kUnit;
+  r.nblk = max(1, (r.len + kUnit - 1) / kUnit - r.blk0);  // a row that sees nothing is written too
+  return r;
+}
+
+__device__ __forceinline__ void read_request(const AttnArgs& a, int b, int& c0, int& c1, int& len) {
+  c0 = c1 = len = 0;
+  if (b < a.B) {
+    c0 = a.cu ? a.cu[b] : b;
+    c1 = a.cu ? a.cu[b + 1] : b + 1;
+    len = a.seq[b];
+  }
+}
+
+// The tile that CTA i began and others end.
+struct Begun {
+  int last;  // the CTA that ends it; -1: none
+  int q0, work, h, tile;
+};
+
+template <typename T, int D, int NT>
+struct __align__(16) Smem {
+  float m[kWarps][8 * NT], l[kWarps][8 * NT];
+  float o[kWarps][8 * NT][D + 4];
+};
+
+// What a warp loads for one step: NS subtiles of 16 positions.
+template <int D, int NT>
+struct Steps {
+  static constexpr int NS = NT == 1 ? 256 / D : (D == 64 ? 2 : 1);
+};
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
+  constexpr int R = 8 * NT, NS = Steps<D, NT>::NS, KC = D / 32, VC = D / 64;
+  __shared__ Smem<T, D, NT> sm;
+  __shared__ int64_t wsum[kWarps], start_rem, total;
+  __shared__ int start_b;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  Begun* begun = reinterpret_cast<Begun*>(a.ws);
+  if (tid == 0) begun[blockIdx.x].last = -1;
+
+  // ---- this CTA's share
+  {
+    const int per = (a.B + kThreads - 1) / kThreads;
+    const int lo = min(tid * per, a.B), hi = min(lo + per, a.B);
+    auto units = [&](int b) {
+      int c0, c1, len;
+      read_request(a, b, c0, c1, len);
+      if (blockIdx.x == 0 && (len < 0 || len > a.max_kv)) atomicOr(&g_attn_status, RNB_STATUS_BAD_INDEX);
+      const Request r = request_of<R>(a, c0, c1, len);
+      return static_cast<int64_t>(r.ntile) * r.nblk * a.Hkv;
+    };
+    int64_t sum = 0;
+    for (int b = lo; b < hi; ++b) sum += units(b);
+    int64_t inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t u = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += u;
+    }
+    if (lane == 31) wsum[warp] = inc;
+    __syncthreads();
+    int64_t base = inc - sum;
+    for (int w = 0; w < warp; ++w) base += wsum[w];
+    if (tid == kThreads - 1) total = base + sum;
+    __syncthreads();
+    const int64_t share = (total + gridDim.x - 1) / gridDim.x, u0 = share * blockIdx.x;
+    if (u0 >= base && u0 < base + sum) {
+      int64_t rem = u0 - base;
+      int b = lo;
+      for (int64_t n = units(b); rem >= n; n = units(b)) {
+        rem -= n;
+        ++b;
+      }
+      start_b = b;
+      start_rem = rem;
+    }
+    __syncthreads();
+  }
+  const int64_t share = (total + gridDim.x - 1) / gridDim.x, u0 = share * blockIdx.x;
+  const int64_t u1 = min(u0 + share, total);
+  if (u0 >= u1) return;
+  int b = start_b;
+  int64_t rem = start_rem;
+  int c0, c1, len;
+  read_request(a, b, c0, c1, len);
+  Request rq = request_of<R>(a, c0, c1, len);
+  read_request(a, b + 1, c0, c1, len);  // one ahead
+
+  for (int64_t u = u0; u < u1;) {
+    const int64_t mine = static_cast<int64_t>(rq.ntile) * rq.nblk * a.Hkv;
+    if (rem >= mine) {
+      rem -= mine;
+      ++b;
+      rq = request_of<R>(a, c0, c1, len);
+      read_request(a, b + 1, c0, c1, len);
+      continue;
+    }
+    const int tile_of = static_cast<int>(rem / rq.nblk), blk = static_cast<int>(rem - static_cast<int64_t>(tile_of) * rq.nblk);
+    const int h = tile_of / rq.ntile, tile = tile_of - h * rq.ntile;
+    const int n = static_cast<int>(min(static_cast<int64_t>(rq.nblk - blk), u1 - u));
+    const int work = rq.rows * a.group;
+
+    // ---- the tile's queries, in K's element order, and each row's positions
+    uint32_t qf[NT][KC][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = tile * R + nt * 8 + g, i = row / a.group, j = row - i * a.group;
+      const T* qp = static_cast<const T*>(a.q) + (rq.q0 + i) * a.q_ts + (h * a.group + j) * a.q_hs + 8 * c;
+#pragma unroll
+      for (int s = 0; s < KC; ++s) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (row < work) v = __ldg(reinterpret_cast<const uint4*>(qp + 32 * s));
+        qf[nt][s][0] = v.x, qf[nt][s][1] = v.y, qf[nt][s][2] = v.z, qf[nt][s][3] = v.w;
+      }
+    }
+    const int p0 = rq.len - rq.rows;  // position of the request's first row
+    int seen_hi[NT][2], seen_lo[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = min(tile * R + nt * 8 + 2 * c + e, work - 1), p = p0 + row / a.group;
+        seen_hi[nt][e] = p;
+        seen_lo[nt][e] = a.window > 0 ? p - a.window + 1 : INT_MIN;
+      }
+    const int first_p = p0 + (tile * R) / a.group, last_p = p0 + min(tile * R + R - 1, work - 1) / a.group;
+    const int all_lo = a.window > 0 ? last_p - a.window + 1 : INT_MIN;    // from here every row sees, up to first_p
+    const int any_lo = a.window > 0 ? first_p - a.window + 1 : INT_MIN;   // before here none does
+    const int s_end = min((rq.blk0 + blk + n) * kUnit, last_p + 1);
+
+    float o[NT][VC][4][4];
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) m[nt][e] = -INFINITY, l[nt][e] = 0.f;
+#pragma unroll
+      for (int s = 0; s < VC; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nt][s][j][e] = 0.f;
+    }
+
+    const int32_t* row_table = a.table + static_cast<int64_t>(b) * a.W;
+    const T* kh = static_cast<const T*>(a.kc) + h * a.kc_hs + g * D + 8 * c;
+    const T* vh = static_cast<const T*>(a.vc) + h * a.vc_hs + 2 * c * D + 8 * g;
+    const int pmask = (1 << a.log2p) - 1;
+    auto pages_of = [&](int s, int (&pid)[NS]) {
+#pragma unroll
+      for (int ns = 0; ns < NS; ++ns) {
+        const int st = s + 16 * ns;
+        pid[ns] = st < s_end ? __ldg(row_table + (st >> a.log2p)) : -1;
+      }
+    };
+    uint4 kr[NS][KC][2], vr[NS][VC][4];
+    auto load_k = [&](int s, const int (&pid)[NS]) {
+#pragma unroll
+      for (int ns = 0; ns < NS; ++ns) {
+        const bool ok = static_cast<uint32_t>(pid[ns]) < static_cast<uint32_t>(a.num_pages);
+        const T* p = kh + (ok ? pid[ns] : 0) * a.kc_ps + ((s + 16 * ns) & pmask) * D;
+#pragma unroll
+        for (int i = 0; i < KC; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            kr[ns][i][e] = make_uint4(0, 0, 0, 0);
+            if (ok) kr[ns][i][e] = ld_stream_v4(p + 32 * i + 8 * e * D);
+          }
+      }
+    };
+    auto load_v = [&](int s, const int (&pid)[NS]) {
+#pragma unroll
+      for (int ns = 0; ns < NS; ++ns) {
+        const bool ok = static_cast<uint32_t>(pid[ns]) < static_cast<uint32_t>(a.num_pages);
+        const T* p = vh + (ok ? pid[ns] : 0) * a.vc_ps + ((s + 16 * ns) & pmask) * D;
+#pragma unroll
+        for (int i = 0; i < VC; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            vr[ns][i][e] = make_uint4(0, 0, 0, 0);
+            if (ok) vr[ns][i][e] = ld_stream_v4(p + 64 * i + ((e & 1) + 8 * (e >> 1)) * D);
+          }
+      }
+    };
+
+    constexpr int kStep = 16 * NS;
+    int s = (rq.blk0 + blk) * kUnit + warp * kStep;
+    int pid[NS], nxt[NS];
+    pages_of(s, pid);
+    load_k(s, pid);
+    load_v(s, pid);
+    pages_of(s + kWarps * kStep, nxt);
+    for (; s < s_end; s += kWarps * kStep) {
+      // S^T
+      float sc[NS][NT][4];
+#pragma unroll
+      for (int ns = 0; ns < NS; ++ns)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < KC; ++i) {
+            const uint4 x = kr[ns][i][0], y = kr[ns][i][1];
+            mma_t<T>(d0, x.x, y.x, x.y, y.y, qf[nt][i][0], qf[nt][i][1]);
+            mma_t<T>(d1, x.z, y.z, x.w, y.w, qf[nt][i][2], qf[nt][i][3]);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[ns][nt][e] = (d0[e] + d1[e]) * a.scale_log2;
+        }
+      int cur[NS];
+      bool whole = s + kStep - 1 <= first_p && s >= all_lo;
+#pragma unroll
+      for (int ns = 0; ns < NS; ++ns) {
+        cur[ns] = pid[ns];
+        whole = whole && static_cast<uint32_t>(cur[ns]) < static_cast<uint32_t>(a.num_pages);
+        pid[ns] = nxt[ns];
+      }
+      const int s_next = s + kWarps * kStep;
+      load_k(s_next, pid);
+      pages_of(s_next + kWarps * kStep, nxt);
+      if (!whole) {
+#pragma unroll
+        for (int ns = 0; ns < NS; ++ns) {
+          const int st = s + 16 * ns;
+          const bool ok = static_cast<uint32_t>(cur[ns]) < static_cast<uint32_t>(a.num_pages);
+          if (!ok && st < s_end && lane == 0) atomicOr(&g_attn_status, RNB_STATUS_BAD_INDEX);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int t = st + g + 8 * (e >> 1);
+              if (!ok || t >= s_end || t > seen_hi[nt][e & 1] || t < seen_lo[nt][e & 1]) sc[ns][nt][e] = -INFINITY;
+            }
+          // values that no row of the tile sees: their bits must not count
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int t = st + 2 * c + (e & 1) + 8 * (e >> 1);
+            if (t >= s_end || t < any_lo) {
+#pragma unroll
+              for (int i = 0; i < VC; ++i) vr[ns][i][e] = make_uint4(0, 0, 0, 0);
+            }
+          }
+        }
+      }
+      // running maximum and sum
+      bool grew = false;
+      float f[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float mx = m[nt][e];
+#pragma unroll
+          for (int ns = 0; ns < NS; ++ns) mx = fmaxf(mx, fmaxf(sc[ns][nt][e], sc[ns][nt][e + 2]));
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+          const float use = mx == -INFINITY ? 0.f : mx;
+          f[nt][e] = ex2(m[nt][e] - use);
+          grew = grew || mx > m[nt][e];
+          m[nt][e] = mx;
+          float add = 0.f;
+#pragma unroll
+          for (int ns = 0; ns < NS; ++ns) {
+            sc[ns][nt][e] = ex2(sc[ns][nt][e] - use);
+            sc[ns][nt][e + 2] = ex2(sc[ns][nt][e + 2] - use);
+            add += sc[ns][nt][e] + sc[ns][nt][e + 2];
+          }
+          l[nt][e] = l[nt][e] * f[nt][e] + add;
+        }
+      if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < VC; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[nt][i][j][e] *= f[nt][e & 1];
+      }
+      // O^T += V^T P^T
+#pragma unroll
+      for (int ns = 0; ns < NS; ++ns) {
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          pb[nt][0] = transpose8(Pair<T>::pack(sc[ns][nt][0], sc[ns][nt][1]));
+          pb[nt][1] = transpose8(Pair<T>::pack(sc[ns][nt][2], sc[ns][nt][3]));
+        }
+#pragma unroll
+        for (int i = 0; i < VC; ++i) {
+          const uint32_t* v0 = &vr[ns][i][0].x;
+          const uint32_t* v1 = &vr[ns][i][1].x;
+          const uint32_t* v2 = &vr[ns][i][2].x;
+          const uint32_t* v3 = &vr[ns][i][3].x;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t a0 = __byte_perm(v0[j], v1[j], 0x5410), a1 = __byte_perm(v0[j], v1[j], 0x7632);
+            const uint32_t a2 = __byte_perm(v2[j], v3[j], 0x5410), a3 = __byte_perm(v2[j], v3[j], 0x7632);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_t<T>(o[nt][i][j], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+          }
+        }
+      }
+      load_v(s_next, pid);
+    }
+
+    // ---- join the four warps
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], d);
+        if (g == 0) {
+          sm.m[warp][nt * 8 + 2 * c + e] = m[nt][e];
+          sm.l[warp][nt * 8 + 2 * c + e] = l[nt][e];
+        }
+#pragma unroll
+        for (int i = 0; i < VC; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<float2*>(&sm.o[warp][nt * 8 + 2 * c + e][64 * i + 8 * g + 2 * j]) =
+                make_float2(o[nt][i][j][e], o[nt][i][j][e + 2]);
+      }
+    __syncthreads();
+    const bool begins = blk == 0, ends = blk + n == rq.nblk;
+    const int part = 2 * blockIdx.x + (begins ? 1 : 0);
+    float* part_ml = reinterpret_cast<float*>(a.ws + a.ml_off) + static_cast<int64_t>(part) * R * 2;
+    float* part_o = reinterpret_cast<float*>(a.ws + a.o_off) + static_cast<int64_t>(part) * R * D;
+    for (int x = tid; x < R * (D / 4); x += kThreads) {
+      const int r = x / (D / 4), d = (x - r * (D / 4)) * 4;
+      float mx = sm.m[0][r];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, sm.m[w][r]);
+      const float use = mx == -INFINITY ? 0.f : mx;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      float ls = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float wf = ex2(sm.m[w][r] - use);
+        const float4 v = *reinterpret_cast<const float4*>(&sm.o[w][r][d]);
+        acc.x = fmaf(v.x, wf, acc.x), acc.y = fmaf(v.y, wf, acc.y);
+        acc.z = fmaf(v.z, wf, acc.z), acc.w = fmaf(v.w, wf, acc.w);
+        ls = fmaf(sm.l[w][r], wf, ls);
+      }
+      if (begins && ends) {
+        const int row = tile * R + r;
+        if (row < work) attn_write_row<T, D>(a, rq.q0 + row / a.group, h * a.group + row % a.group, d, acc, mx, ls);
+      } else {
+        *reinterpret_cast<float4*>(part_o + r * D + d) = acc;
+        if (d == 0) part_ml[2 * r] = mx, part_ml[2 * r + 1] = ls;
+      }
+    }
+    if (begins && !ends && tid == 0) {
+      const int64_t tile_end = u + (rq.nblk - blk);  // first unit behind the tile
+      Begun bg;
+      bg.last = static_cast<int>((tile_end - 1) / share);
+      bg.q0 = rq.q0, bg.work = work, bg.h = h, bg.tile = tile;
+      begun[blockIdx.x] = bg;
+    }
+    __syncthreads();  // the join's shared memory is free again
+    rem += n;
+    u += n;
+  }
+  griddep_launch_dependents();
+}
+
+// Block (i, r): row r of the tile that CTA i of the kernel above began, from the
+// parts of CTAs i .. last, in order.
+template <typename T, int D, int R>
+__global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
+  constexpr int kCols = D / 4, kWays = 256 / kCols;
+  __shared__ float4 acc_s[kWays][kCols];
+  __shared__ float red[8], lred[kWays];
+  griddep_wait();
+  const Begun bg = reinterpret_cast<const Begun*>(a.ws)[blockIdx.x];
+  const int r = blockIdx.y, row = bg.tile * R + r;
+  if (bg.last < 0 || row >= bg.work) return;
+  const int tid = threadIdx.x, n = bg.last - static_cast<int>(blockIdx.x) + 1;
+  const float* ml = reinterpret_cast<const float*>(a.ws + a.ml_off);
+  const float* po = reinterpret_cast<const float*>(a.ws + a.o_off);
+  auto part = [&](int i) { return static_cast<int64_t>(2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * R + r; };
+  float mx = -INFINITY;
+  for (int i = tid; i < n; i += 256) mx = fmaxf(mx, ml[2 * part(i)]);
+  mx = warp_max(mx);
+  if ((tid & 31) == 0) red[tid >> 5] = mx;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) mx = fmaxf(mx, red[w]);
+  const float use = mx == -INFINITY ? 0.f : mx;
+  const int col = tid % kCols, way = tid / kCols;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float ls = 0.f;
+  for (int i = way; i < n; i += kWays) {
+    const int64_t p = part(i);
+    const float f = ex2(ml[2 * p] - use);
+    const float4 v = *reinterpret_cast<const float4*>(po + p * D + 4 * col);
+    acc.x = fmaf(v.x, f, acc.x), acc.y = fmaf(v.y, f, acc.y);
+    acc.z = fmaf(v.z, f, acc.z), acc.w = fmaf(v.w, f, acc.w);
+    ls = fmaf(ml[2 * p + 1], f, ls);
+  }
+  acc_s[way][col] = acc;
+  if (col == 0) lred[way] = ls;
+  __syncthreads();
+  if (way == 0) {
+#pragma unroll
+    for (int w = 1; w < kWays; ++w) {
+      const float4 v = acc_s[w][col];
+      acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+      ls += lred[w];
+    }
+    ls = lred[0];
+#pragma unroll
+    for (int w = 1; w < kWays; ++w) ls += lred[w];
+    attn_write_row<T, D>(a, bg.q0 + row / a.group, bg.h * a.group + row % a.group, 4 * col, acc, mx, ls);
+  }
+}
+
+struct Plan {
+  int R, grid;
+  size_t ml_off, o_off, bytes;
+};
+
+Plan plan_of(const rnb_attn_desc* d, const rnb_kv_cache* c, int sms) {
+  Plan p;
+  const int64_t group = d->n_q_heads / c->n_kv_heads;
+  const int64_t most = d->max_q > 0 ? d->max_q : d->T > d->B ? d->T : 1;  // rows of one request
+  // 8 rows where all fit (half the registers and products of 16); heads of 256
+  // always, since 16 of them do not fit the registers
+  p.R = c->head_dim == 256 || most * group <= 8 ? 8 : 16;
+  p.grid = 2 * sms;
+  p.ml_off = (sizeof(Begun) * p.grid + 255) & ~size_t(255);
+  p.o_off = (p.ml_off + 2u * p.grid * p.R * 2 * sizeof(float) + 255) & ~size_t(255);
+  p.bytes = p.o_off + 2u * p.grid * p.R * static_cast<size_t>(c->head_dim) * sizeof(float);
+  return p;
+}
+
+template <typename T, int D, int NT>
+int run_few(AttnArgs a, int grid, cudaStream_t st) {
+  k_attn_few<T, D, NT><<<grid, kThreads, 0, st>>>(a);
+  int rc = launch_status("rnb_paged_attention");
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid, 8 * NT);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_attn_join<T, D, 8 * NT>, a);
+  if (e != cudaSuccess) return fail(RNB_ERR_CUDA, std::string("rnb_paged_attention join: ") + cudaGetErrorString(e));
+  return RNB_OK;
+}
+
+template <typename T>
+int run_few_typed(const AttnArgs& a, int D, int R, int grid, cudaStream_t st) {
+  if (D == 256) return run_few<T, 256, 1>(a, grid, st);
+  if (D == 128) return R == 8 ? run_few<T, 128, 1>(a, grid, st) : run_few<T, 128, 2>(a, grid, st);
+  return R == 8 ? run_few<T, 64, 1>(a, grid, st) : run_few<T, 64, 2>(a, grid, st);
+}
+
+int check_attn(const rnb_attn_desc* d, const rnb_kv_cache* c) {
+  if (!d) return fail(RNB_ERR_INVALID, "rnb_paged_attention: descriptor is NULL");
+  int rc = check_cache(c, "rnb_paged_attention");
+  if (rc) return rc;
+  if (d->B < 0 || d->T < 0) return fail(RNB_ERR_INVALID, "rnb_paged_attention: B and T must be >= 0");
+  if (d->n_q_heads <= 0 || d->n_q_heads % c->n_kv_heads)
+    return fail(RNB_ERR_INVALID, "rnb_paged_attention: n_q_heads must be a positive multiple of n_kv_heads");
+  if (static_cast<int64_t>(d->T) * d->n_q_heads > INT32_MAX)
+    return fail(RNB_ERR_INVALID, "rnb_paged_attention: T * n_q_heads must be below 2^31");
+  if (d->table_cols <= 0) return fail(RNB_ERR_INVALID, "rnb_paged_attention: table_cols must be positive");
+  if (d->max_q < 0 || d->window < 0)
+    return fail(RNB_ERR_INVALID, "rnb_paged_attention: max_q and window must be >= 0");
+  if (!(d->scale > 0.f) || !(d->scale < INFINITY))
+    return fail(RNB_ERR_INVALID, "rnb_paged_attention: scale must be positive and finite");
+  const int64_t st[4] = {d->q_token_stride, d->q_head_stride, d->gate_token_stride, d->gate_head_stride};
+  for (int64_t v : st)
+    if (v < 0 || v % 8) return fail(RNB_ERR_INVALID, "rnb_paged_attention: strides must be multiples of 8 elements");
+  return RNB_OK;
+}
+
+}  // namespace
+
+int attn_status_take(uint32_t* bits, cudaStream_t st) { return status_take(g_attn_status, bits, st); }
+
+}  // namespace rnb
+
+extern "C" {
+
+int rnb_paged_attention_workspace_size(const rnb_attn_desc* d, const rnb_kv_cache* cache, size_t* bytes) {
+  using namespace rnb;
+  if (!bytes) return fail(RNB_ERR_INVALID, "bytes must be non-NULL");
+  int rc = check_attn(d, cache);
+  if (rc) return rc;
+  const int sms = dev_info().sms;
+  *bytes = plan_of(d, cache, sms > 0 ? sms : 148).bytes;
+  return RNB_OK;
+}
+
+int rnb_paged_attention(const rnb_attn_desc* d, const rnb_kv_cache* cache, const void* q, const void* gate,
+                        const int32_t* table, const int32_t* seq_lens, const int32_t* cu_q, void* out, float* lse,
+                        void* ws, size_t ws_bytes, void* stream) {
+  using namespace rnb;
+  int rc = check_attn(d, cache);
+  if (rc) return rc;
+  if (!cu_q && d->T != d->B)
+    return fail(RNB_ERR_INVALID, "rnb_paged_attention: without cu_q every request has one row (T == B)");
+  if (d->B == 0 || d->T == 0) return RNB_OK;
+  if (!q || !out || !table || !seq_lens)
+    return fail(RNB_ERR_INVALID, "rnb_paged_attention: q, out, table and seq_lens must be non-NULL");
+  if (!aligned16(q) || !aligned16(gate) || !aligned16(out) || !aligned16(ws))
+    return fail(RNB_ERR_ALIGN, "rnb_paged_attention: q, gate, out and the workspace must be 16-byte aligned");
+  if ((rc = check_device())) return rc;
+  const Plan p = plan_of(d, cache, dev_info().sms);
+  if (!ws || ws_bytes < p.bytes)
+    return fail(RNB_ERR_WORKSPACE, "rnb_paged_attention: the workspace needs " + std::to_string(p.bytes) + " bytes");
+
+  AttnArgs a{};
+  a.q = q, a.gate = gate, a.out = out, a.lse = lse;
+  a.kc = cache->k, a.vc = cache->v;
+  a.table = table, a.seq = seq_lens, a.cu = cu_q;
+  a.ws = static_cast<char*>(ws), a.ml_off = p.ml_off, a.o_off = p.o_off;
+  a.q_ts = d->q_token_stride, a.q_hs = d->q_head_stride;
+  a.g_ts = d->gate_token_stride, a.g_hs = d->gate_head_stride;
+  a.kc_ps = cache->k_page_stride, a.kc_hs = cache->k_head_stride;
+  a.vc_ps = cache->v_page_stride, a.vc_hs = cache->v_head_stride;
+  a.B = d->B, a.T = d->T, a.W = d->table_cols;
+  a.Hq = d->n_q_heads, a.Hkv = cache->n_kv_heads, a.group = a.Hq / a.Hkv;
+  while ((1 << a.log2p) < cache->page_size) ++a.log2p;
+  a.num_pages = cache->num_pages, a.window = d->window;
+  const int64_t kv = static_cast<int64_t>(d->table_cols) * cache->page_size;
+  a.max_kv = static_cast<int>(kv < INT32_MAX - 4096 ? kv : INT32_MAX - 4096);  // steps ahead stay in 31 bits
+  a.few_rows = INT32_MAX;
+  a.scale_log2 = d->scale * 1.4426950408889634f;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return cache->dtype == RNB_DTYPE_BF16 ? run_few_typed<__nv_bfloat16>(a, cache->head_dim, p.R, p.grid, st)
+                                        : run_few_typed<__half>(a, cache->head_dim, p.R, p.grid, st);
+}
+
+}  // extern "C"

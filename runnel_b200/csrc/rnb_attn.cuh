@@ -1,0 +1,42 @@
+// rnb_attn.cuh -- arguments and the output epilogue of the paged-attention kernels.
+#pragma once
+
+#include <stdint.h>
+
+#include "rnb_kv.cuh"
+
+namespace rnb {
+
+struct AttnArgs {
+  const void *q, *gate, *kc, *vc;
+  const int32_t *table, *seq, *cu;
+  void* out;
+  float* lse;
+  char* ws;
+  size_t ml_off, o_off;
+  int64_t q_ts, q_hs, g_ts, g_hs, kc_ps, kc_hs, vc_ps, vc_hs;
+  float scale_log2;  // scale * log2(e): softmax in powers of two
+  int B, T, W, Hq, Hkv, group, log2p, num_pages, window, max_kv;
+  int few_rows;  // requests with rows * group below this are the few-row kernel's
+};
+
+// Four consecutive elements of one output row: o / l, times sigmoid(gate),
+// rounded once; the row's lse = ln 2 (m + log2 l) from the thread with d == 0.
+template <typename T, int D>
+__device__ __forceinline__ void attn_write_row(const AttnArgs& a, int t, int head, int d, float4 o, float m, float l) {
+  const float inv = l > 0.f ? 1.0f / l : 0.f;
+  float v[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+  if (a.gate) {
+    const uint2 w =
+        *reinterpret_cast<const uint2*>(static_cast<const T*>(a.gate) + t * a.g_ts + head * a.g_hs + d);
+    const float2 g0 = Pair<T>::unpack(w.x), g1 = Pair<T>::unpack(w.y);
+    v[0] /= 1.f + __expf(-g0.x), v[1] /= 1.f + __expf(-g0.y);
+    v[2] /= 1.f + __expf(-g1.x), v[3] /= 1.f + __expf(-g1.y);
+  }
+  const int64_t row = static_cast<int64_t>(t) * a.Hq + head;
+  *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + row * D + d) =
+      make_uint2(Pair<T>::pack(v[0], v[1]), Pair<T>::pack(v[2], v[3]));
+  if (a.lse && d == 0) a.lse[row] = l > 0.f ? 0.6931471805599453f * (m + log2f(l)) : -INFINITY;
+}
+
+}  // namespace rnb

@@ -1,0 +1,87 @@
+// rnb_kv.cuh -- what the attention-side units (page plan, rotary append,
+// paged attention) share: checks of a cache descriptor and the 16-bit types.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <string>
+
+#include "rnb_common.cuh"
+#include "rnb_internal.h"
+#include "rnb_moe.h"
+
+namespace rnb {
+
+// RNB_OK, or an error with its message: shapes, strides and alignment of a
+// paged cache.
+inline int check_cache(const rnb_kv_cache* c, const char* fn) {
+  const std::string f = std::string(fn) + ": ";
+  if (!c) return fail(RNB_ERR_INVALID, f + "the cache must be non-NULL");
+  if (c->dtype != RNB_DTYPE_BF16 && c->dtype != RNB_DTYPE_F16)
+    return fail(RNB_ERR_INVALID, f + "the cache's dtype must be RNB_DTYPE_BF16 or RNB_DTYPE_F16");
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+    return fail(RNB_ERR_INVALID, f + "head_dim must be 64, 128 or 256");
+  const int P = c->page_size;
+  if (P < 16 || P > 256 || (P & (P - 1)))
+    return fail(RNB_ERR_INVALID, f + "page_size must be 16, 32, 64, 128 or 256");
+  if (c->num_pages <= 0 || c->n_kv_heads <= 0 || c->n_kv_heads > 65535)
+    return fail(RNB_ERR_INVALID, f + "num_pages must be positive and n_kv_heads in [1, 65535]");
+  if (static_cast<int64_t>(c->num_pages) * P > INT32_MAX)
+    return fail(RNB_ERR_INVALID, f + "num_pages * page_size must be below 2^31");
+  if (!c->k || !c->v) return fail(RNB_ERR_INVALID, f + "cache k and v must be non-NULL");
+  if (!aligned16(c->k) || !aligned16(c->v)) return fail(RNB_ERR_ALIGN, f + "cache k and v must be 16-byte aligned");
+  const int64_t st[4] = {c->k_page_stride, c->k_head_stride, c->v_page_stride, c->v_head_stride};
+  for (int64_t v : st)
+    if (v < 0 || v % 8) return fail(RNB_ERR_INVALID, f + "cache strides must be multiples of 8 elements");
+  return RNB_OK;
+}
+
+inline int launch_status(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(RNB_ERR_CUDA, std::string(what) + " launch: " + cudaGetErrorString(e));
+  return RNB_OK;
+}
+
+// Reads and clears one unit's device status word (synchronises the stream).
+int rope_status_take(uint32_t* bits, cudaStream_t st);
+int attn_status_take(uint32_t* bits, cudaStream_t st);
+
+template <typename Sym>
+inline int status_take(Sym& word, uint32_t* bits, cudaStream_t st) {
+  const uint32_t zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbolAsync(bits, word, sizeof zero, 0, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e == cudaSuccess) e = cudaMemcpyToSymbolAsync(word, &zero, sizeof zero, 0, cudaMemcpyHostToDevice, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e != cudaSuccess) return fail(RNB_ERR_CUDA, std::string("rnb_kv_status: ") + cudaGetErrorString(e));
+  return RNB_OK;
+}
+
+// The two 16-bit types: packing (round to nearest even) and unpacking of pairs.
+template <typename T>
+struct Pair;
+template <>
+struct Pair<__nv_bfloat16> {
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t v) {
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+  }
+};
+template <>
+struct Pair<__half> {
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t v) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&v));
+  }
+};
+
+}  // namespace rnb
