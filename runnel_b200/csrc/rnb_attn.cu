@@ -43,6 +43,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kUnit = 64;  // positions
+constexpr int kManyRows = 64;  // rows * group from which a request is the many-row kernel's
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -627,6 +628,14 @@ int rnb_paged_attention(const rnb_attn_desc* d, const rnb_kv_cache* cache, const
   a.few_rows = INT32_MAX;
   a.scale_log2 = d->scale * 1.4426950408889634f;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int64_t most = cu_q ? (d->max_q > 0 ? d->max_q : d->T) : 1;
+  if (cu_q && most * a.group >= kManyRows) {
+    PromptMaps maps;
+    if (prepare_prompt(cache, &maps)) {
+      a.few_rows = kManyRows;
+      if ((rc = run_prompt(a, cache, maps, st))) return rc;
+    }
+  }
   return cache->dtype == RNB_DTYPE_BF16 ? run_few_typed<__nv_bfloat16>(a, cache->head_dim, p.R, p.grid, st)
                                         : run_few_typed<__half>(a, cache->head_dim, p.R, p.grid, st);
 }

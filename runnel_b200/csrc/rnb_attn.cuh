@@ -1,6 +1,7 @@
 // rnb_attn.cuh -- arguments and the output epilogue of the paged-attention kernels.
 #pragma once
 
+#include <cuda.h>
 #include <stdint.h>
 
 #include "rnb_kv.cuh"
@@ -19,6 +20,16 @@ struct AttnArgs {
   int B, T, W, Hq, Hkv, group, log2p, num_pages, window, max_kv;
   int few_rows;  // requests with rows * group below this are the few-row kernel's
 };
+
+// The many-row kernel (rnb_attn_prompt.cu): TMA maps of a cache, and a launch
+// for the requests with rows * group >= a.few_rows.  prepare_prompt is false
+// where the encoder does not take the cache's layout.
+struct PromptMaps {
+  CUtensorMap k, v;
+  int k_box, v_box;  // rows a copy
+};
+bool prepare_prompt(const rnb_kv_cache* c, PromptMaps* p);
+int run_prompt(const AttnArgs& a, const rnb_kv_cache* c, const PromptMaps& p, cudaStream_t st);
 
 // Four consecutive elements of one output row: o / l, times sigmoid(gate),
 // rounded once; the row's lse = ln 2 (m + log2 l) from the thread with d == 0.

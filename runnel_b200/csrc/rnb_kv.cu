@@ -286,11 +286,12 @@ int rnb_kv_status(uint32_t* status, void* stream) {
   int rc = check_device();
   if (rc) return rc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  uint32_t v[3] = {0, 0, 0};
+  uint32_t v[4] = {0, 0, 0, 0};
   if ((rc = status_take(g_kv_status, &v[0], st))) return rc;
   if ((rc = rope_status_take(&v[1], st))) return rc;
   if ((rc = attn_status_take(&v[2], st))) return rc;
-  *status = v[0] | v[1] | v[2];
+  if ((rc = prompt_status_take(&v[3], st))) return rc;
+  *status = v[0] | v[1] | v[2] | v[3];
   return RNB_OK;
 }
 

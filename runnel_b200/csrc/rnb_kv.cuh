@@ -48,6 +48,7 @@ inline int launch_status(const char* what) {
 // Reads and clears one unit's device status word (synchronises the stream).
 int rope_status_take(uint32_t* bits, cudaStream_t st);
 int attn_status_take(uint32_t* bits, cudaStream_t st);
+int prompt_status_take(uint32_t* bits, cudaStream_t st);
 
 template <typename Sym>
 inline int status_take(Sym& word, uint32_t* bits, cudaStream_t st) {
