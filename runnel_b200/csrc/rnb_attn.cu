@@ -631,7 +631,7 @@ int rnb_paged_attention(const rnb_attn_desc* d, const rnb_kv_cache* cache, const
   const int64_t most = cu_q ? (d->max_q > 0 ? d->max_q : d->T) : 1;
   if (cu_q && most * a.group >= kManyRows) {
     PromptMaps maps;
-    if (prepare_prompt(cache, &maps)) {
+    if (prepare_prompt(a, cache, &maps)) {
       a.few_rows = kManyRows;
       if ((rc = run_prompt(a, cache, maps, st))) return rc;
     }

@@ -21,14 +21,15 @@ struct AttnArgs {
   int few_rows;  // requests with rows * group below this are the few-row kernel's
 };
 
-// The many-row kernel (rnb_attn_prompt.cu): TMA maps of a cache, and a launch
-// for the requests with rows * group >= a.few_rows.  prepare_prompt is false
-// where the encoder does not take the cache's layout.
+// The many-row kernel (rnb_attn_prompt.cu): TMA maps of the call's tensors, and
+// a launch for the requests with rows * group >= a.few_rows.  prepare_prompt is
+// false where the kernel or the encoder does not take the layout.
 struct PromptMaps {
-  CUtensorMap k, v;
-  int k_box, v_box;  // rows a copy
+  CUtensorMap k, v, q, gate, out;
+  int k_box, v_box;  // cache rows a copy
+  int tokens;        // tokens a row tile
 };
-bool prepare_prompt(const rnb_kv_cache* c, PromptMaps* p);
+bool prepare_prompt(const AttnArgs& a, const rnb_kv_cache* c, PromptMaps* p);
 int run_prompt(const AttnArgs& a, const rnb_kv_cache* c, const PromptMaps& p, cudaStream_t st);
 
 // Four consecutive elements of one output row: o / l, times sigmoid(gate),

@@ -1,9 +1,10 @@
 // rnb_attn_prompt.cu -- attention over the paged cache for requests with many
 // query rows (prompts), on the 5th-generation tensor cores.
 //
-// One CTA takes 128 (head_dim 256) or 256 query rows of one key head: rows are
-// (token, query head of the group) pairs, so the group's heads share every key
-// and value that is loaded.  Over blocks of 128 positions
+// One CTA takes one (head_dim 256) or two tiles of up to 128 query rows of one
+// key head: a tile is floor(128 / group) tokens with the group's query heads, so
+// that the heads share every key and value that is loaded, and queries, gates
+// and outputs are boxes of (tokens, heads, elements) that TMA moves.  Over blocks of 128 positions
 //     S = Q K^T,  P = 2^(scale log2e S - m),  O += P V,  l += rowsum P
 // with S, P and O in tensor memory: S is 128 fp32 columns, P overwrites it as
 // 16-bit pairs and is the A operand of the second product from there, so no
@@ -46,29 +47,54 @@ constexpr uint64_t kWaitNs = 1000000000ull;
 template <int D>
 struct Cfg {
   static constexpr int NQ = D == 256 ? 1 : 2;              // row tiles a CTA
-  static constexpr int kRows = 128 * NQ;
   static constexpr int kThreads = 128 + 128 * NQ;          // loader, issuer, two idle warps; softmax warpgroups
   static constexpr int UPT = D == 256 ? 2 : 1;             // ring units a K or V block
   static constexpr int kUnit = kBlk * D * 2 / UPT;         // bytes
   static constexpr int VR = kBlk / UPT;                    // V rows a unit (all of D)
   static constexpr int KD = D / UPT;                       // K elements a unit (all rows)
   static constexpr int NST = D == 64 ? 8 : 5;
-  static constexpr int kQBytes = kRows * D * 2;
+  static constexpr int kQBytes = 128 * NQ * D * 2;
   static constexpr int kSmem = kQBytes + NST * kUnit + 1024;
   static constexpr int kTmemO = 256;                       // S slots at columns 0 and 128
 };
 
-// D[tmem] (+)= A[tmem] * B[smem]; issued by one thread.
-__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
-                                            uint32_t accumulate) {
+// D[tmem] (+)= A * B, A from shared memory (ss) or tensor memory (ts).  The
+// whole warp executes these with one lane's predicate set: in a branch of one
+// lane the operands would have to be moved to uniform registers one by one,
+// which cost 115 cycles a product.
+__device__ __forceinline__ void umma_ss(uint32_t leader, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                        uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t"
-      ".reg .pred p;\n\t"
+      ".reg .pred p, e;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t"
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
       "}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0), "r"(0), "r"(0), "r"(0)
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader)
       : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc,
+                                        uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, e;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, e;\n\t}"
+      : "=r"(r));
+  return r;
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
@@ -100,6 +126,32 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
       "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
       "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
+}
+
+// 3-D tiled TMA store of a box in shared memory; its group is committed and
+// waited for (until the box is read) by the issuing thread.
+__device__ __forceinline__ void tma_store_3d(const void* tmap, uint32_t src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(tmap),
+               "r"(x), "r"(y), "r"(z), "r"(src)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit_and_wait_read() {
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+
+// A barrier of 128 threads: whether `ok` holds for all of them.
+__device__ __forceinline__ bool all_of_128(int id, bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %2, 0;\n\t"
+      "barrier.cta.red.and.pred q, %1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(static_cast<uint32_t>(ok))
+      : "memory");
+  return r != 0;
 }
 
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -146,6 +198,8 @@ __device__ __forceinline__ float ex2(float x) {
 struct Bars {
   uint64_t full[8], empty[8];   // ring units
   uint64_t q_full;              // Q in shared memory
+  uint64_t q_done;              // every product with Q done
+  uint64_t g_full;              // the gates where Q was
   uint64_t s_full[2], p_full[2];  // slots: S written, P written (S read)
   uint64_t o_done[2];           // row tiles: a P V product done
   uint64_t o_last[2];           // row tiles: the last one done
@@ -154,29 +208,37 @@ struct Bars {
 
 template <typename T, int D>
 __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
-    k_attn_prompt(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                  int k_box, int v_box) {
+    k_attn_prompt(const AttnArgs a, const __grid_constant__ PromptMaps maps) {
   using C = Cfg<D>;
   extern __shared__ char raw[];
   __shared__ Bars bars;
   __shared__ uint32_t tmem_slot;
   __shared__ int64_t wsum[C::kThreads / 32];
-  __shared__ int found_b, found_tile;
+  __shared__ int found[5];  // request, tile, first row, rows, length
+  __shared__ bool gave_up;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   char* ring = smem + C::kQBytes;
+  const int tt = maps.tokens;            // tokens a row tile
+  const int cta_tokens = tt * C::NQ;
 
-  // ---- which request and tile: tiles of a request from its end (the longest first)
+  // ---- which request and tokens: tiles of a request from its end (the longest first)
   const int h = blockIdx.x % a.Hkv;
   const int64_t want = blockIdx.x / a.Hkv;
   {
-    if (tid == 0) found_b = -1;
+    if (tid == 0) {
+      found[0] = -1;
+      // after a wait that gave up, until the status is read: a grid of CTAs that
+      // each wait their second would hold the device for minutes
+      gave_up = *const_cast<volatile uint32_t*>(&g_prompt_status) & RNB_STATUS_TIMEOUT;
+    }
     const int per = (a.B + C::kThreads - 1) / C::kThreads;
     const int lo = min(tid * per, a.B), hi = min(lo + per, a.B);
+    int c0 = 0, c1 = 0, ln = 0;
     auto tiles = [&](int b) {
-      const int c0 = min(max(a.cu[b], 0), a.T), c1 = min(max(a.cu[b + 1], c0), a.T);
-      const int work = (c1 - c0) * a.group;
-      return work >= a.few_rows ? (work + C::kRows - 1) / C::kRows : 0;
+      c0 = min(max(a.cu[b], 0), a.T), c1 = min(max(a.cu[b + 1], c0), a.T);
+      ln = a.seq[b];
+      return (c1 - c0) * a.group >= a.few_rows ? (c1 - c0 + cta_tokens - 1) / cta_tokens : 0;
     };
     int64_t sum = 0;
     for (int b = lo; b < hi; ++b) sum += tiles(b);
@@ -193,42 +255,39 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     if (want >= base && want < base + sum) {
       int64_t rem = want - base;
       int b = lo;
-      int n = tiles(b);
+      int n = per == 1 ? static_cast<int>(sum) : tiles(b);
       while (rem >= n) {
         rem -= n;
         n = tiles(++b);
       }
-      found_b = b;
-      found_tile = n - 1 - static_cast<int>(rem);
+      found[0] = b, found[1] = n - 1 - static_cast<int>(rem);
+      found[2] = c0, found[3] = c1 - c0, found[4] = ln;
     }
     __syncthreads();
   }
-  const int b = found_b, tile = found_tile;
-  // (after a wait that gave up, until the status is read: a grid of CTAs that
-  // each wait their second would hold the device for minutes)
-  if (b < 0 || (*const_cast<volatile uint32_t*>(&g_prompt_status) & RNB_STATUS_TIMEOUT)) return;
-  const int q0 = min(max(a.cu[b], 0), a.T), rows = min(max(a.cu[b + 1], q0), a.T) - q0;
-  const int len_raw = a.seq[b], len = min(max(len_raw, 0), a.max_kv);
-  const int work = rows * a.group, p0 = len - rows;
-  const int row0 = tile * C::kRows, row_end = min(row0 + C::kRows, work);
-  const int first_p = p0 + row0 / a.group, last_p = p0 + (row_end - 1) / a.group;
+  const int b = found[0], tile = found[1], q0 = found[2], rows = found[3];
+  if (b < 0 || gave_up) return;
+  const int len = min(max(found[4], 0), a.max_kv);
+  const int p0 = len - rows;                          // position of the request's first token
+  const int tok0 = tile * cta_tokens, tok_end = min(tok0 + cta_tokens, rows);
+  const int first_p = p0 + tok0, last_p = p0 + tok_end - 1;
   const int any_lo = a.window > 0 ? max(first_p - a.window + 1, 0) : 0;
   const int kv_end = max(last_p + 1, 0);
   const int blk0 = any_lo / kBlk;
   const int nblk = max((kv_end + kBlk - 1) / kBlk - blk0, 0);
   const int32_t* row_table = a.table + static_cast<int64_t>(b) * a.W;
-
-  // page ids out of range in this tile's positions: their masks need the table
-  int bad = 0;
-  for (int j = (any_lo >> a.log2p) + tid; j < (kv_end + (1 << a.log2p) - 1) >> a.log2p; j += C::kThreads)
-    bad |= static_cast<uint32_t>(__ldg(row_table + j)) >= static_cast<uint32_t>(a.num_pages);
+  // a row tile in shared memory: 64-element columns of 128 rows, 128-byte swizzle
+  constexpr int kCol = 128 * 128;
+  const uint32_t q_bytes = C::NQ * (D / 64) * static_cast<uint32_t>(tt * a.group) * 128;
 
   if (tid == 0) {
     for (int i = 0; i < C::NST; ++i) {
       mbar_init(&bars.full[i], 1);
       mbar_init(&bars.empty[i], 1);
     }
-    mbar_init(&bars.q_full, 4 * C::NQ);
+    mbar_init(&bars.q_full, 1);
+    mbar_init(&bars.q_done, 1);
+    mbar_init(&bars.g_full, 1);
     mbar_init(&bars.drained, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.s_full[i], 1);
@@ -237,18 +296,28 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
       mbar_init(&bars.o_last[i], 1);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    if (len_raw != len) atomicOr(&g_prompt_status, RNB_STATUS_BAD_INDEX);
+    if (found[4] != len) atomicOr(&g_prompt_status, RNB_STATUS_BAD_INDEX);
   }
   if (warp == 2) {
     tmem_alloc(&tmem_slot, 512);
     tmem_relinquish();
   }
   tc_fence_before();
-  bad = __syncthreads_or(bad);
+  __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  if (bad && tid == 0) atomicOr(&g_prompt_status, RNB_STATUS_BAD_INDEX);
   bool alive = true;
+  // queries or gates of the CTA's tiles; tokens behind the last are read as
+  // zeros or as another request's, whose rows are not used
+  auto load_tiles = [&](const CUtensorMap* map, uint64_t* bar) {
+    if (lane == 0) mbar_arrive_expect_tx(bar, q_bytes);
+    __syncwarp();
+    if (lane < C::NQ * (D / 64)) {
+      const int q = lane / (D / 64), c = lane - q * (D / 64);
+      tma_load_3d(smem_u32(smem) + lane * kCol, map, 64 * c, h * a.group, q0 + tok0 + q * tt, smem_u32(bar));
+    }
+    __syncwarp();
+  };
   const int jobs = nblk * C::NQ;  // job k: slot k & 1; two row tiles a block, or a block a job
 
   if (warp == 0) {
@@ -261,7 +330,10 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
       int id = a.num_pages;
       if (lane < kBlk / 16 && t < kv_end && (t | pmask) >= any_lo) {  // its page holds seen positions
         const int p = __ldg(row_table + (t >> a.log2p));
-        if (static_cast<uint32_t>(p) < static_cast<uint32_t>(a.num_pages)) id = p;
+        if (static_cast<uint32_t>(p) < static_cast<uint32_t>(a.num_pages))
+          id = p;
+        else
+          atomicOr(&g_prompt_status, RNB_STATUS_BAD_INDEX);
       }
       return id;
     };
@@ -273,7 +345,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
         const uint32_t bar = smem_u32(&bars.full[st]), dst = rbase + st * C::kUnit;
         if (lane == 0) mbar_arrive_expect_tx(&bars.full[st], C::kUnit);
         __syncwarp();
-        const int box = is_k ? k_box : v_box;
+        const int box = is_k ? maps.k_box : maps.v_box;
         const int rows_u = is_k ? kBlk : C::VR, skip = is_k ? 0 : part * C::VR;
         const int nbox = rows_u / box;
         const int page = __shfl_sync(0xffffffffu, id, ((skip + lane * box) >> 4) & 31);
@@ -281,13 +353,14 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
           const int t = blk * kBlk + skip + lane * box;
           const int nch = is_k ? C::KD / 64 : D / 64, ch0 = is_k ? part * (C::KD / 64) : 0;
           for (int c = 0; c < nch; ++c)
-            tma_load_4d(dst + (c * rows_u + lane * box) * 128, is_k ? static_cast<const void*>(&kmap) : &vmap,
+            tma_load_4d(dst + (c * rows_u + lane * box) * 128, is_k ? static_cast<const void*>(&maps.k) : &maps.v,
                         (ch0 + c) * 64, t & pmask, h, page, bar);
         }
         __syncwarp();
       }
     };
     if (nblk > 0) {
+      load_tiles(&maps.q, &bars.q_full);
       if (C::NQ == 2) {
         int id = ids(blk0);
         for (int i = 0; i < nblk && alive; ++i) {
@@ -308,14 +381,20 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
         }
       }
     }
+    if (a.gate && alive && nblk > 0) alive = wait_on(&bars.q_done, 0);
+    if (a.gate && alive) load_tiles(&maps.gate, &bars.g_full);
     // no copy may be in flight when the CTA ends
+    if (nblk > 0) wait_on(&bars.q_full, 0);
+    if (a.gate && alive) wait_on(&bars.g_full, 0);
     for (int v = max(u - C::NST, 0); v < u; ++v) wait_on(&bars.full[v % C::NST], (v / C::NST) & 1);
   } else if (warp == 1) {
     // ---- issuer
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     const uint32_t id_s = umma_idesc_f16(128, kBlk, kBf16);
     const uint32_t id_o = umma_idesc_f16(128, D, kBf16) | (1u << 16);  // B is MN-major
-    const uint32_t rbase = smem_u32(ring), qbase = smem_u32(smem);
+    const uint32_t rbase = smem_u32(ring);
+    const uint64_t qdesc = umma_desc_sw128(smem_u32(smem));
+    const uint32_t leader = elect_one();
     // ring units of block i: with two row tiles K0 V0 K1 V1 ..., else K0 K1 V0 K2 V1 ...
     auto unit_k = [&](int i) { return (C::NQ == 2 ? 2 * i : i == 0 ? 0 : 2 * i - 1) * C::UPT; };
     auto unit_v = [&](int i) { return (C::NQ == 2 ? 2 * i + 1 : min(2 + 2 * i, 2 * nblk - 1)) * C::UPT; };
@@ -326,16 +405,15 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
         alive = wait_on(&bars.full[st], (u / C::NST) & 1);
         if (!alive) return;
         tc_fence_after();
-        if (lane == 0) {
+        const uint64_t qd = qdesc + ((q * (D / 64) + part * (C::KD / 64)) * (128 * 128 >> 4));
+        const uint64_t kd = umma_desc_sw128(rbase + st * C::kUnit);
 #pragma unroll
-          for (int c = 0; c < C::KD / 64; ++c)
+        for (int c = 0; c < C::KD / 64; ++c)
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-              const int ch = part * (C::KD / 64) + c;
-              const uint32_t qa = qbase + (q * (D / 64) + ch) * 128 * 128 + 32 * s;
-              const uint32_t ka = rbase + st * C::kUnit + c * kBlk * 128 + 32 * s;
-              umma_f16(tmem + (k & 1) * 128, umma_desc_sw128(qa), umma_desc_sw128(ka), id_s, (ch | s) != 0);
-            }
+          for (int s = 0; s < 4; ++s)
+            umma_ss(leader, tmem + (k & 1) * 128, qd + ((c * 128 * 128 + 32 * s) >> 4),
+                    kd + ((c * kBlk * 128 + 32 * s) >> 4), id_s, part != 0 || (c | s) != 0);
+        if (leader) {
           if (C::NQ == 1 || q == 1) umma_commit(smem_u32(&bars.empty[st]));
           if (part == C::UPT - 1) umma_commit(smem_u32(&bars.s_full[k & 1]));
         }
@@ -364,13 +442,12 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
           if (!alive) return;
         }
         tc_fence_after();
-        if (lane == 0) {
+        const uint64_t vd = umma_desc_mn(rbase + st * C::kUnit, C::VR * 128);
 #pragma unroll
-          for (int s = 0; s < C::VR / 16; ++s) {
-            const uint32_t va = rbase + st * C::kUnit + s * 16 * 128;
-            umma_f16_ts(tmem + C::kTmemO + q * D, tmem + (k & 1) * 128 + (part * C::VR + s * 16) / 2,
-                        umma_desc_mn(va, C::VR * 128), id_o, i != 0 || part != 0 || s != 0);
-          }
+        for (int s = 0; s < C::VR / 16; ++s)
+          umma_ts(leader, tmem + C::kTmemO + q * D, tmem + (k & 1) * 128 + (part * C::VR + s * 16) / 2,
+                  vd + (s * 16 * 128 >> 4), id_o, i != 0 || part != 0 || s != 0);
+        if (leader) {
           if (C::NQ == 1 || q == 1) umma_commit(smem_u32(&bars.empty[st]));
           if (part == C::UPT - 1) umma_commit(smem_u32(i + 1 < nblk ? &bars.o_done[q] : &bars.o_last[q]));
         }
@@ -385,41 +462,40 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
       for (int k = 0; k < jobs && alive; ++k) {
         issue_o(k);
         if (alive && k + 2 < jobs) issue_s(k + 2);
+        if (k + 3 == jobs || (k == 0 && jobs < 3)) {  // the last product with Q is issued
+          if (leader) umma_commit(smem_u32(&bars.q_done));
+          __syncwarp();
+        }
       }
       // no product may be in flight when the tensor memory is given back
-      if (lane == 0) umma_commit(smem_u32(&bars.drained));
+      if (leader) umma_commit(smem_u32(&bars.drained));
       __syncwarp();
       wait_on(&bars.drained, 0);
     }
   } else if (warp >= 4) {
     // ---- softmax: a thread is a row of tile wg
-    const int wg = (warp - 4) >> 2, r = tid - 128 - 128 * wg;
-    const int row = row0 + wg * 128 + r;
-    // Q into the K-major layout, coalesced over the rows' elements
-    for (int x = r; x < 128 * (D / 8); x += 128) {
-      const int qr = x / (D / 8), e = (x - qr * (D / 8)) * 8, rr = row0 + wg * 128 + qr;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (rr < work) {
-        const int i = rr / a.group, j = rr - i * a.group;
-        v = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (q0 + i) * a.q_ts +
-                                                 (h * a.group + j) * a.q_hs + e));
-      }
-      *reinterpret_cast<uint4*>(smem + (wg * (D / 64) + (e >> 6)) * 128 * 128 + sw128_offset(qr, e & 63)) = v;
-    }
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&bars.q_full);
-
-    const int pos = p0 + min(row, work - 1) / a.group;
+    const int wg = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;  // row tile and row in it
+    const int wt0 = tok0 + wg * tt, wt_end = min(wt0 + tt, rows);  // its tokens (none: wt0 >= rows)
+    const int tok = wt0 + r / a.group, head = h * a.group + r % a.group;
+    const bool in = r < tt * a.group && tok < rows;
+    const int pos = p0 + min(tok, tok_end - 1);
     const int see_lo = a.window > 0 ? pos - a.window + 1 : INT_MIN;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_o = tmem + C::kTmemO + wg * D + lane_base;
     // positions that all rows of this warpgroup's tile see
-    const int wg_first = p0 + min(row0 + wg * 128, work - 1) / a.group;
-    const int wg_last = p0 + min(row0 + wg * 128 + 127, work - 1) / a.group;
-    const int all_lo = a.window > 0 ? wg_last - a.window + 1 : INT_MIN;
+    const int wg_first = p0 + min(wt0, tok_end - 1);
+    const int all_lo = a.window > 0 ? p0 + min(wt0 + tt, tok_end) - a.window : INT_MIN;
+    // lanes 0-7 watch the page ids of the next block's subtiles of 16 positions
+    auto page_at = [&](int i) {
+      const int t = (blk0 + i) * kBlk + 16 * lane;
+      return lane < kBlk / 16 && t < kv_end ? __ldg(row_table + (t >> a.log2p)) : 0;
+    };
+    int page = nblk > 0 ? page_at(0) : 0;
     float m = -INFINITY, l = 0.f;
     for (int i = 0; i < nblk && alive; ++i) {
+      const uint32_t bad =
+          __ballot_sync(0xffffffffu, static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.num_pages));
+      if (i + 1 < nblk) page = page_at(i + 1);
       const int k = C::NQ == 2 ? 2 * i + wg : i, slot = k & 1;
       const uint32_t t_s = tmem + slot * 128 + lane_base;
       alive = wait_on(&bars.s_full[slot], (k >> 1) & 1);
@@ -442,23 +518,19 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int e = 0; e < 32; e += 16) {
-              const int t = t0 + 32 * c + e;
-              if (t < kv_end && static_cast<uint32_t>(__ldg(row_table + (t >> a.log2p))) >=
-                                    static_cast<uint32_t>(a.num_pages)) {
-#pragma unroll
-                for (int f = 0; f < 16; ++f) v[c][e + f] = __float_as_uint(-INFINITY);
-              }
-            }
+            for (int e = 0; e < 32; ++e)
+              if (bad >> (2 * c + (e >> 4)) & 1) v[c][e] = __float_as_uint(-INFINITY);
         }
       }
-      float mx = __uint_as_float(v[0][0]);
+      float mc[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < 4; ++c) {
+        mc[c] = __uint_as_float(v[c][0]);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) mx = fmaxf(mx, __uint_as_float(v[c][e]));
-      mx *= a.scale_log2;
-      if (__any_sync(0xffffffffu, mx > m + 8.f)) {
+        for (int e = 1; e < 32; ++e) mc[c] = fmaxf(mc[c], __uint_as_float(v[c][e]));
+      }
+      const float mx = fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3])) * a.scale_log2;
+      if (__any_sync(0xffffffffu, in && mx > m + 8.f)) {  // (what rows out of use hold must not matter)
         const float to = fmaxf(m, mx);
         const float f = ex2(m - (to == -INFINITY ? 0.f : to));
         m = to;
@@ -481,6 +553,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
         }
       }
       const float use = m == -INFINITY ? 0.f : m;
+      float l0 = 0.f, l1 = 0.f;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         uint32_t p[16];
@@ -488,11 +561,12 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
         for (int e = 0; e < 16; ++e) {
           const float x = ex2(fmaf(__uint_as_float(v[c][2 * e]), a.scale_log2, -use));
           const float y = ex2(fmaf(__uint_as_float(v[c][2 * e + 1]), a.scale_log2, -use));
-          l += x + y;
+          l0 += x, l1 += y;
           p[e] = Pair<T>::pack(x, y);
         }
         tmem_st16(t_s + 16 * c, p);
       }
+      l += l0 + l1;
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -503,25 +577,61 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     // parity only tells neighbouring phases apart)
     if (alive && nblk > 0) alive = wait_on(&bars.o_last[wg], 0);
     tc_fence_after();
+    if (a.gate && alive) alive = wait_on(&bars.g_full, 0);
     if (alive) {
-      const int t = q0 + row / a.group, head = h * a.group + row % a.group;
+      // in place of Q, or of the gates that have come there
+      char* base = smem + wg * (D / 64) * kCol;
+      const float inv = l > 0.f ? 1.0f / l : 0.f;
+      if (a.lse && in)
+        a.lse[static_cast<int64_t>(q0 + tok) * a.Hq + head] = l > 0.f ? 0.6931471805599453f * (m + log2f(l)) : -INFINITY;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = 0;
         if (nblk > 0) {
           tmem_ld32(t_o + 32 * c, o);
           tmem_wait_ld();
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0;
         }
-        if (row < work) {
+        char* at = base + (c >> 1) * kCol;
 #pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            attn_write_row<T, D>(a, t, head, 32 * c + e,
-                                 make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]),
-                                             __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3])),
-                                 m, l);
+        for (int x = 0; x < 4; ++x) {
+          uint4* piece = reinterpret_cast<uint4*>(at + sw128_offset(r, (c & 1) * 32 + 8 * x));
+          uint32_t w[4];
+          uint4 gw = make_uint4(0, 0, 0, 0);
+          if (a.gate) gw = *piece;
+          const uint32_t gu[4] = {gw.x, gw.y, gw.z, gw.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float y0 = __uint_as_float(o[8 * x + 2 * e]) * inv, y1 = __uint_as_float(o[8 * x + 2 * e + 1]) * inv;
+            if (a.gate) {
+              const float2 gf = Pair<T>::unpack(gu[e]);
+              y0 = __fdividef(y0, 1.f + __expf(-gf.x)), y1 = __fdividef(y1, 1.f + __expf(-gf.y));
+            }
+            w[e] = Pair<T>::pack(y0, y1);
+          }
+          *piece = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      fence_proxy_async_smem();
+    }
+    // the warpgroup's four warps, those that gave up among them
+    if (all_of_128(1 + wg, alive)) {
+      const char* base = smem + wg * (D / 64) * kCol;
+      if (wt0 + tt <= rows) {
+        if (r == 0) {
+          for (int c = 0; c < D / 64; ++c)
+            tma_store_3d(&maps.out, smem_u32(base + c * kCol), 64 * c, h * a.group, q0 + wt0);
+          bulk_commit_and_wait_read();
+        }
+      } else {
+        // the request's last tile: only its own rows
+        const int n = max(wt_end - wt0, 0) * a.group;
+        for (int x = r; x < n * (D / 8); x += 128) {
+          const int rr = x / (D / 8), e = (x - rr * (D / 8)) * 8, i = rr / a.group;
+          *reinterpret_cast<uint4*>(static_cast<T*>(a.out) +
+                                    (static_cast<int64_t>(q0 + wt0 + i) * a.Hq + h * a.group + rr - i * a.group) * D + e) =
+              *reinterpret_cast<const uint4*>(base + (e >> 6) * kCol + sw128_offset(rr, e & 63));
         }
       }
     }
@@ -534,16 +644,15 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
 }
 
 template <typename T, int D>
-int launch_prompt(const AttnArgs& a, const rnb_kv_cache* cache, const CUtensorMap& km, const CUtensorMap& vm, int kbox,
-                  int vbox, cudaStream_t st) {
+int launch_prompt(const AttnArgs& a, const PromptMaps& maps, cudaStream_t st) {
   using C = Cfg<D>;
   const cudaError_t e = cudaFuncSetAttribute(k_attn_prompt<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (e != cudaSuccess) return fail(RNB_ERR_CUDA, std::string("rnb_paged_attention: ") + cudaGetErrorString(e));
   // as many tiles as there can be: CTAs without one end at once
-  const int64_t most = (static_cast<int64_t>(a.T) * a.group + C::kRows - 1) / C::kRows;
-  const int64_t tiles = most + (a.B < static_cast<int64_t>(a.T) ? a.B : a.T);
+  const int64_t per = static_cast<int64_t>(maps.tokens) * C::NQ;
+  const int64_t tiles = (a.T + per - 1) / per + (a.B < a.T ? a.B : a.T);
   if (tiles * a.Hkv > INT32_MAX) return fail(RNB_ERR_INVALID, "rnb_paged_attention: too many rows");
-  k_attn_prompt<T, D><<<static_cast<unsigned>(tiles * a.Hkv), C::kThreads, C::kSmem, st>>>(a, km, vm, kbox, vbox);
+  k_attn_prompt<T, D><<<static_cast<unsigned>(tiles * a.Hkv), C::kThreads, C::kSmem, st>>>(a, maps);
   return launch_status("rnb_paged_attention");
 }
 
@@ -558,29 +667,43 @@ bool encode_cache(CUtensorMap* m, const rnb_kv_cache* c, const void* base, int64
   return encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, base, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// [T][n_q_heads][D] in boxes of (tokens, the group's heads, 64 elements)
+bool encode_rows(CUtensorMap* m, const AttnArgs& a, const void* base, int D, int64_t ts, int64_t hs, int tokens) {
+  const uint64_t dims[3] = {static_cast<uint64_t>(D), static_cast<uint64_t>(a.Hq), static_cast<uint64_t>(a.T)};
+  const uint64_t str[2] = {a.Hq > 1 ? 2u * static_cast<uint64_t>(hs) : 2u * D,
+                           a.T > 1 ? 2u * static_cast<uint64_t>(ts) : 2u * D * a.Hq};
+  const uint32_t box[3] = {64, static_cast<uint32_t>(a.group), static_cast<uint32_t>(tokens)};
+  return encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, base, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 }  // namespace
 
 int prompt_status_take(uint32_t* bits, cudaStream_t st) { return status_take(g_prompt_status, bits, st); }
 
-bool prepare_prompt(const rnb_kv_cache* c, PromptMaps* p) {
+bool prepare_prompt(const AttnArgs& a, const rnb_kv_cache* c, PromptMaps* p) {
+  if (a.group > 128) return false;
   const int D = c->head_dim, P = c->page_size;
+  p->tokens = 128 / a.group;
   p->k_box = P < kBlk ? P : kBlk;
   const int vr = D == 256 ? Cfg<256>::VR : kBlk;
   p->v_box = P < vr ? P : vr;
   return encode_cache(&p->k, c, c->k, c->k_page_stride, c->k_head_stride, p->k_box) &&
-         encode_cache(&p->v, c, c->v, c->v_page_stride, c->v_head_stride, p->v_box);
+         encode_cache(&p->v, c, c->v, c->v_page_stride, c->v_head_stride, p->v_box) &&
+         encode_rows(&p->q, a, a.q, D, a.q_ts, a.q_hs, p->tokens) &&
+         encode_rows(&p->out, a, a.out, D, static_cast<int64_t>(a.Hq) * D, D, p->tokens) &&
+         (!a.gate || encode_rows(&p->gate, a, a.gate, D, a.g_ts, a.g_hs, p->tokens));
 }
 
 int run_prompt(const AttnArgs& a, const rnb_kv_cache* c, const PromptMaps& p, cudaStream_t st) {
   const int D = c->head_dim;
   if (c->dtype == RNB_DTYPE_BF16) {
-    if (D == 64) return launch_prompt<__nv_bfloat16, 64>(a, c, p.k, p.v, p.k_box, p.v_box, st);
-    if (D == 128) return launch_prompt<__nv_bfloat16, 128>(a, c, p.k, p.v, p.k_box, p.v_box, st);
-    return launch_prompt<__nv_bfloat16, 256>(a, c, p.k, p.v, p.k_box, p.v_box, st);
+    if (D == 64) return launch_prompt<__nv_bfloat16, 64>(a, p, st);
+    if (D == 128) return launch_prompt<__nv_bfloat16, 128>(a, p, st);
+    return launch_prompt<__nv_bfloat16, 256>(a, p, st);
   }
-  if (D == 64) return launch_prompt<__half, 64>(a, c, p.k, p.v, p.k_box, p.v_box, st);
-  if (D == 128) return launch_prompt<__half, 128>(a, c, p.k, p.v, p.k_box, p.v_box, st);
-  return launch_prompt<__half, 256>(a, c, p.k, p.v, p.k_box, p.v_box, st);
+  if (D == 64) return launch_prompt<__half, 64>(a, p, st);
+  if (D == 128) return launch_prompt<__half, 128>(a, p, st);
+  return launch_prompt<__half, 256>(a, p, st);
 }
 
 }  // namespace rnb
