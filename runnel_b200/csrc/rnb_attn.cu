@@ -622,9 +622,10 @@ int rnb_paged_attention(const rnb_attn_desc* d, const rnb_kv_cache* cache, const
   a.B = d->B, a.T = d->T, a.W = d->table_cols;
   a.Hq = d->n_q_heads, a.Hkv = cache->n_kv_heads, a.group = a.Hq / a.Hkv;
   while ((1 << a.log2p) < cache->page_size) ++a.log2p;
-  a.num_pages = cache->num_pages, a.window = d->window;
+  a.num_pages = cache->num_pages;
   const int64_t kv = static_cast<int64_t>(d->table_cols) * cache->page_size;
   a.max_kv = static_cast<int>(kv < INT32_MAX - 4096 ? kv : INT32_MAX - 4096);  // steps ahead stay in 31 bits
+  a.window = d->window < a.max_kv ? d->window : 0;
   a.few_rows = INT32_MAX;
   a.scale_log2 = d->scale * 1.4426950408889634f;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -4,9 +4,9 @@
 // One CTA takes one (head_dim 256) or two tiles of up to 128 query rows of one
 // key head: a tile is floor(128 / group) tokens with the group's query heads, so
 // that the heads share every key and value that is loaded, and queries, gates
-// and outputs are boxes of (tokens, heads, elements) that TMA moves.  Over blocks of 128 positions
+// and outputs are boxes of (tokens, heads, elements) that TMA moves.  Over blocks of positions
 //     S = Q K^T,  P = 2^(scale log2e S - m),  O += P V,  l += rowsum P
-// with S, P and O in tensor memory: S is 128 fp32 columns, P overwrites it as
+// with S, P and O in tensor memory: S is a column a position, P overwrites it as
 // 16-bit pairs and is the A operand of the second product from there, so no
 // probability passes through shared memory.  A thread owns a row: its maximum
 // and sum need no exchange.
@@ -14,10 +14,12 @@
 // * The maximum is lazy: m only moves when a row's maximum exceeds it by more
 //   than 8 (P stays below 2^8, in range of both types), so O is hardly ever
 //   rescaled after the first blocks.
-// * Two S slots keep the tensor cores fed: while the softmax of one slot runs,
-//   the products of the other do.  With head_dim <= 128 the slots are two row
-//   tiles with a softmax warpgroup each; with 256, where one O fills half the tensor
-//   memory, they are two successive blocks of one tile.
+// * Slots of S keep the tensor cores and the softmax apart: S of later blocks is
+//   computed before P of this one is done.  With head_dim <= 128 there are two row
+//   tiles with a softmax warpgroup and two slots of 64 positions each (one slot of 128
+//   each made a warpgroup wait for its own two products every block: 3900
+//   cycles a 128 positions); with 256, where one O fills half the tensor memory, two
+//   slots of 128 positions of one tile.
 // * Keys and values come by TMA page by page into a ring of 128-byte-swizzled
 //   units, K as the K-major and V as the MN-major operand, both as they lie in the
 //   cache.  Pages behind the request's end (and ids out of range) are fetched at
@@ -41,21 +43,22 @@ namespace {
 
 __device__ uint32_t g_prompt_status;
 
-constexpr int kBlk = 128;  // positions a block
 constexpr uint64_t kWaitNs = 1000000000ull;
 
 template <int D>
 struct Cfg {
   static constexpr int NQ = D == 256 ? 1 : 2;              // row tiles a CTA
+  static constexpr int BN = 128;                           // positions a block
+  static constexpr int NS = 256 / BN;                      // S slots, of BN columns, in 256
   static constexpr int kThreads = 128 + 128 * NQ;          // loader, issuer, two idle warps; softmax warpgroups
   static constexpr int UPT = D == 256 ? 2 : 1;             // ring units a K or V block
-  static constexpr int kUnit = kBlk * D * 2 / UPT;         // bytes
-  static constexpr int VR = kBlk / UPT;                    // V rows a unit (all of D)
+  static constexpr int kUnit = BN * D * 2 / UPT;           // bytes
+  static constexpr int VR = BN / UPT;                      // V rows a unit (all of D)
   static constexpr int KD = D / UPT;                       // K elements a unit (all rows)
-  static constexpr int NST = D == 64 ? 8 : 5;
+  static constexpr int NST = D == 64 ? 8 : 5;              // ring units
   static constexpr int kQBytes = 128 * NQ * D * 2;
   static constexpr int kSmem = kQBytes + NST * kUnit + 1024;
-  static constexpr int kTmemO = 256;                       // S slots at columns 0 and 128
+  static constexpr int kTmemO = 256;
 };
 
 // D[tmem] (+)= A * B, A from shared memory (ss) or tensor memory (ts).  The
@@ -195,12 +198,35 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)),
+        "l"(reinterpret_cast<const uint64_t&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+  return d;
+}
+
 struct Bars {
-  uint64_t full[8], empty[8];   // ring units
+  uint64_t full[10], empty[10];   // ring units
   uint64_t q_full;              // Q in shared memory
   uint64_t q_done;              // every product with Q done
   uint64_t g_full;              // the gates where Q was
-  uint64_t s_full[2], p_full[2];  // slots: S written, P written (S read)
+  uint64_t s_full[4], p_full[4];  // slots: S written, P written (S read)
   uint64_t o_done[2];           // row tiles: a P V product done
   uint64_t o_last[2];           // row tiles: the last one done
   uint64_t drained;             // every product of the CTA done
@@ -273,8 +299,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
   const int first_p = p0 + tok0, last_p = p0 + tok_end - 1;
   const int any_lo = a.window > 0 ? max(first_p - a.window + 1, 0) : 0;
   const int kv_end = max(last_p + 1, 0);
-  const int blk0 = any_lo / kBlk;
-  const int nblk = max((kv_end + kBlk - 1) / kBlk - blk0, 0);
+  const int blk0 = any_lo / C::BN;
+  const int nblk = max((kv_end + C::BN - 1) / C::BN - blk0, 0);
   const int32_t* row_table = a.table + static_cast<int64_t>(b) * a.W;
   // a row tile in shared memory: 64-element columns of 128 rows, 128-byte swizzle
   constexpr int kCol = 128 * 128;
@@ -289,9 +315,11 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     mbar_init(&bars.q_done, 1);
     mbar_init(&bars.g_full, 1);
     mbar_init(&bars.drained, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < C::NS; ++i) {
       mbar_init(&bars.s_full[i], 1);
       mbar_init(&bars.p_full[i], 4);
+    }
+    for (int i = 0; i < C::NQ; ++i) {
       mbar_init(&bars.o_done[i], 1);
       mbar_init(&bars.o_last[i], 1);
     }
@@ -318,7 +346,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     }
     __syncwarp();
   };
-  const int jobs = nblk * C::NQ;  // job k: slot k & 1; two row tiles a block, or a block a job
+  const int jobs = nblk * C::NQ;  // job k: block k / NQ of row tile k % NQ, in slot k % NS
 
   if (warp == 0) {
     // ---- loader: units in the order in which the issuer uses them
@@ -326,9 +354,9 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     const int pmask = (1 << a.log2p) - 1;
     int u = 0;
     auto ids = [&](int blk) {  // lane l: the page of the block's subtile l of 16 positions
-      const int t = blk * kBlk + 16 * lane;
+      const int t = blk * C::BN + 16 * lane;
       int id = a.num_pages;
-      if (lane < kBlk / 16 && t < kv_end && (t | pmask) >= any_lo) {  // its page holds seen positions
+      if (lane < C::BN / 16 && t < kv_end && (t | pmask) >= any_lo) {  // its page holds seen positions
         const int p = __ldg(row_table + (t >> a.log2p));
         if (static_cast<uint32_t>(p) < static_cast<uint32_t>(a.num_pages))
           id = p;
@@ -346,11 +374,11 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
         if (lane == 0) mbar_arrive_expect_tx(&bars.full[st], C::kUnit);
         __syncwarp();
         const int box = is_k ? maps.k_box : maps.v_box;
-        const int rows_u = is_k ? kBlk : C::VR, skip = is_k ? 0 : part * C::VR;
+        const int rows_u = is_k ? C::BN : C::VR, skip = is_k ? 0 : part * C::VR;
         const int nbox = rows_u / box;
         const int page = __shfl_sync(0xffffffffu, id, ((skip + lane * box) >> 4) & 31);
         if (lane < nbox) {
-          const int t = blk * kBlk + skip + lane * box;
+          const int t = blk * C::BN + skip + lane * box;
           const int nch = is_k ? C::KD / 64 : D / 64, ch0 = is_k ? part * (C::KD / 64) : 0;
           for (int c = 0; c < nch; ++c)
             tma_load_4d(dst + (c * rows_u + lane * box) * 128, is_k ? static_cast<const void*>(&maps.k) : &maps.v,
@@ -361,24 +389,14 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     };
     if (nblk > 0) {
       load_tiles(&maps.q, &bars.q_full);
-      if (C::NQ == 2) {
-        int id = ids(blk0);
-        for (int i = 0; i < nblk && alive; ++i) {
-          const int next = i + 1 < nblk ? ids(blk0 + i + 1) : 0;
-          load(true, blk0 + i, id);
-          load(false, blk0 + i, id);
-          id = next;
-        }
-      } else {
-        int id = ids(blk0), next = nblk > 1 ? ids(blk0 + 1) : 0;
-        load(true, blk0, id);
-        for (int i = 0; i < nblk && alive; ++i) {
-          const int ahead = i + 2 < nblk ? ids(blk0 + i + 2) : 0;
-          if (i + 1 < nblk) load(true, blk0 + i + 1, next);
-          load(false, blk0 + i, id);
-          id = next;
-          next = ahead;
-        }
+      int id = ids(blk0), next = nblk > 1 ? ids(blk0 + 1) : 0;
+      load(true, blk0, id);
+      for (int i = 0; i < nblk && alive; ++i) {
+        const int ahead = i + 2 < nblk ? ids(blk0 + i + 2) : 0;
+        if (i + 1 < nblk) load(true, blk0 + i + 1, next);
+        load(false, blk0 + i, id);
+        id = next;
+        next = ahead;
       }
     }
     if (a.gate && alive && nblk > 0) alive = wait_on(&bars.q_done, 0);
@@ -390,16 +408,16 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
   } else if (warp == 1) {
     // ---- issuer
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-    const uint32_t id_s = umma_idesc_f16(128, kBlk, kBf16);
+    const uint32_t id_s = umma_idesc_f16(128, C::BN, kBf16);
     const uint32_t id_o = umma_idesc_f16(128, D, kBf16) | (1u << 16);  // B is MN-major
     const uint32_t rbase = smem_u32(ring);
     const uint64_t qdesc = umma_desc_sw128(smem_u32(smem));
     const uint32_t leader = elect_one();
-    // ring units of block i: with two row tiles K0 V0 K1 V1 ..., else K0 K1 V0 K2 V1 ...
-    auto unit_k = [&](int i) { return (C::NQ == 2 ? 2 * i : i == 0 ? 0 : 2 * i - 1) * C::UPT; };
-    auto unit_v = [&](int i) { return (C::NQ == 2 ? 2 * i + 1 : min(2 + 2 * i, 2 * nblk - 1)) * C::UPT; };
+    // ring units of block i: K0 K1 V0 K2 V1 ...
+    auto unit_k = [&](int i) { return (i == 0 ? 0 : 2 * i - 1) * C::UPT; };
+    auto unit_v = [&](int i) { return min(2 + 2 * i, 2 * nblk - 1) * C::UPT; };
     auto issue_s = [&](int k) {
-      const int i = C::NQ == 2 ? k >> 1 : k, q = C::NQ == 2 ? k & 1 : 0;
+      const int i = k / C::NQ, q = k % C::NQ;
       for (int part = 0; part < C::UPT && alive; ++part) {
         const int u = unit_k(i) + part, st = u % C::NST;
         alive = wait_on(&bars.full[st], (u / C::NST) & 1);
@@ -411,22 +429,22 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
         for (int c = 0; c < C::KD / 64; ++c)
 #pragma unroll
           for (int s = 0; s < 4; ++s)
-            umma_ss(leader, tmem + (k & 1) * 128, qd + ((c * 128 * 128 + 32 * s) >> 4),
-                    kd + ((c * kBlk * 128 + 32 * s) >> 4), id_s, part != 0 || (c | s) != 0);
+            umma_ss(leader, tmem + (k % C::NS) * C::BN, qd + ((c * 128 * 128 + 32 * s) >> 4),
+                    kd + ((c * C::BN * 128 + 32 * s) >> 4), id_s, part != 0 || (c | s) != 0);
         if (leader) {
           if (C::NQ == 1 || q == 1) umma_commit(smem_u32(&bars.empty[st]));
-          if (part == C::UPT - 1) umma_commit(smem_u32(&bars.s_full[k & 1]));
+          if (part == C::UPT - 1) umma_commit(smem_u32(&bars.s_full[k % C::NS]));
         }
         __syncwarp();
       }
     };
     auto issue_o = [&](int k) {
-      const int i = C::NQ == 2 ? k >> 1 : k, q = C::NQ == 2 ? k & 1 : 0;
+      const int i = k / C::NQ, q = k % C::NQ;
       for (int part = 0; part < C::UPT && alive; ++part) {
         const int u = unit_v(i) + part, st = u % C::NST;
         alive = wait_on(&bars.full[st], (u / C::NST) & 1);
         if (!alive) return;
-        const int t0 = (blk0 + i) * kBlk + part * C::VR;
+        const int t0 = (blk0 + i) * C::BN + part * C::VR;
         if (q == 0 && (t0 + C::VR > kv_end || t0 < any_lo)) {
           // rows that no query row of the tile sees may hold any bits: 0 * NaN must not count
           for (int r = 0; r < C::VR; ++r)
@@ -438,14 +456,14 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
           __syncwarp();
         }
         if (part == 0) {
-          alive = wait_on(&bars.p_full[k & 1], (k >> 1) & 1);
+          alive = wait_on(&bars.p_full[k % C::NS], (k / C::NS) & 1);
           if (!alive) return;
         }
         tc_fence_after();
         const uint64_t vd = umma_desc_mn(rbase + st * C::kUnit, C::VR * 128);
 #pragma unroll
         for (int s = 0; s < C::VR / 16; ++s)
-          umma_ts(leader, tmem + C::kTmemO + q * D, tmem + (k & 1) * 128 + (part * C::VR + s * 16) / 2,
+          umma_ts(leader, tmem + C::kTmemO + q * D, tmem + (k % C::NS) * C::BN + (part * C::VR + s * 16) / 2,
                   vd + (s * 16 * 128 >> 4), id_o, i != 0 || part != 0 || s != 0);
         if (leader) {
           if (C::NQ == 1 || q == 1) umma_commit(smem_u32(&bars.empty[st]));
@@ -457,12 +475,11 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     if (jobs > 0) {
       alive = wait_on(&bars.q_full, 0);
       tc_fence_after();
-      if (alive) issue_s(0);
-      if (alive && jobs > 1) issue_s(1);
+      for (int k = 0; k < min(C::NS, jobs) && alive; ++k) issue_s(k);
       for (int k = 0; k < jobs && alive; ++k) {
         issue_o(k);
-        if (alive && k + 2 < jobs) issue_s(k + 2);
-        if (k + 3 == jobs || (k == 0 && jobs < 3)) {  // the last product with Q is issued
+        if (alive && k + C::NS < jobs) issue_s(k + C::NS);
+        if (k + C::NS + 1 == jobs || (k == 0 && jobs <= C::NS)) {  // the last product with Q is issued
           if (leader) umma_commit(smem_u32(&bars.q_done));
           __syncwarp();
         }
@@ -479,16 +496,16 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     const int tok = wt0 + r / a.group, head = h * a.group + r % a.group;
     const bool in = r < tt * a.group && tok < rows;
     const int pos = p0 + min(tok, tok_end - 1);
-    const int see_lo = a.window > 0 ? pos - a.window + 1 : INT_MIN;
+    const int see_lo = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_o = tmem + C::kTmemO + wg * D + lane_base;
     // positions that all rows of this warpgroup's tile see
     const int wg_first = p0 + min(wt0, tok_end - 1);
     const int all_lo = a.window > 0 ? p0 + min(wt0 + tt, tok_end) - a.window : INT_MIN;
-    // lanes 0-7 watch the page ids of the next block's subtiles of 16 positions
+    // the first lanes watch the page ids of the next block's subtiles of 16 positions
     auto page_at = [&](int i) {
-      const int t = (blk0 + i) * kBlk + 16 * lane;
-      return lane < kBlk / 16 && t < kv_end ? __ldg(row_table + (t >> a.log2p)) : 0;
+      const int t = (blk0 + i) * C::BN + 16 * lane;
+      return lane < C::BN / 16 && t < kv_end ? __ldg(row_table + (t >> a.log2p)) : 0;
     };
     int page = nblk > 0 ? page_at(0) : 0;
     float m = -INFINITY, l = 0.f;
@@ -496,40 +513,47 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
       const uint32_t bad =
           __ballot_sync(0xffffffffu, static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.num_pages));
       if (i + 1 < nblk) page = page_at(i + 1);
-      const int k = C::NQ == 2 ? 2 * i + wg : i, slot = k & 1;
-      const uint32_t t_s = tmem + slot * 128 + lane_base;
-      alive = wait_on(&bars.s_full[slot], (k >> 1) & 1);
+      const int k = C::NQ * i + wg, slot = k % C::NS;
+      const uint32_t t_s = tmem + slot * C::BN + lane_base;
+      alive = wait_on(&bars.s_full[slot], (k / C::NS) & 1);
       if (!alive) break;
       tc_fence_after();
-      uint32_t v[4][32];
+      constexpr int NC = C::BN / 32;
+      uint32_t v[NC][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(t_s + 32 * c, v[c]);
+      for (int c = 0; c < NC; ++c) tmem_ld32(t_s + 32 * c, v[c]);
       tmem_wait_ld();
-      const int t0 = (blk0 + i) * kBlk;
-      if (bad || t0 + kBlk - 1 > wg_first || t0 < all_lo) {
+      const int t0 = (blk0 + i) * C::BN;
+      if (bad || t0 + C::BN - 1 > wg_first || t0 < all_lo) {
+        const int hi = pos - t0, lo = see_lo - t0;
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < NC; ++c)
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const int t = t0 + 32 * c + e;
-            if (t > pos || t < see_lo) v[c][e] = __float_as_uint(-INFINITY);
-          }
-        if (bad) {
+          for (int e = 0; e < 32; ++e)
+            if (32 * c + e > hi) v[c][e] = __float_as_uint(-INFINITY);
+        if (bad || t0 < all_lo) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (bad >> (2 * c + (e >> 4)) & 1) v[c][e] = __float_as_uint(-INFINITY);
+              if (32 * c + e < lo || (bad >> (2 * c + (e >> 4)) & 1)) v[c][e] = __float_as_uint(-INFINITY);
         }
       }
-      float mc[4];
+      float mc[NC][2];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        mc[c] = __uint_as_float(v[c][0]);
+      for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int e = 1; e < 32; ++e) mc[c] = fmaxf(mc[c], __uint_as_float(v[c][e]));
-      }
-      const float mx = fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3])) * a.scale_log2;
+        for (int y = 0; y < 2; ++y) {
+          mc[c][y] = __uint_as_float(v[c][16 * y]);
+#pragma unroll
+          for (int e = 1; e < 15; e += 2)
+            mc[c][y] = max3(mc[c][y], __uint_as_float(v[c][16 * y + e]), __uint_as_float(v[c][16 * y + e + 1]));
+          mc[c][y] = fmaxf(mc[c][y], __uint_as_float(v[c][16 * y + 15]));
+        }
+      float mx = fmaxf(mc[0][0], mc[0][1]);
+#pragma unroll
+      for (int c = 1; c < NC; ++c) mx = max3(mx, mc[c][0], mc[c][1]);
+      mx *= a.scale_log2;
       if (__any_sync(0xffffffffu, in && mx > m + 8.f)) {  // (what rows out of use hold must not matter)
         const float to = fmaxf(m, mx);
         const float f = ex2(m - (to == -INFINITY ? 0.f : to));
@@ -553,20 +577,25 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
         }
       }
       const float use = m == -INFINITY ? 0.f : m;
-      float l0 = 0.f, l1 = 0.f;
+      const float2 scale2 = make_float2(a.scale_log2, a.scale_log2), use2 = make_float2(-use, -use);
+      float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < NC; ++c) {
         uint32_t p[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float x = ex2(fmaf(__uint_as_float(v[c][2 * e]), a.scale_log2, -use));
-          const float y = ex2(fmaf(__uint_as_float(v[c][2 * e + 1]), a.scale_log2, -use));
-          l0 += x, l1 += y;
-          p[e] = Pair<T>::pack(x, y);
+          const float2 x =
+              fma2(make_float2(__uint_as_float(v[c][2 * e]), __uint_as_float(v[c][2 * e + 1])), scale2, use2);
+          const float2 y = make_float2(ex2(x.x), ex2(x.y));
+          if (e & 1)
+            sum1 = add2(sum1, y);
+          else
+            sum0 = add2(sum0, y);
+          p[e] = Pair<T>::pack(y.x, y.y);
         }
         tmem_st16(t_s + 16 * c, p);
       }
-      l += l0 + l1;
+      l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -684,9 +713,11 @@ bool prepare_prompt(const AttnArgs& a, const rnb_kv_cache* c, PromptMaps* p) {
   if (a.group > 128) return false;
   const int D = c->head_dim, P = c->page_size;
   p->tokens = 128 / a.group;
-  p->k_box = P < kBlk ? P : kBlk;
-  const int vr = D == 256 ? Cfg<256>::VR : kBlk;
+  const int bn = D == 256 ? Cfg<256>::BN : Cfg<128>::BN;
+  p->k_box = P < bn ? P : bn;
+  const int vr = D == 256 ? Cfg<256>::VR : Cfg<128>::VR;
   p->v_box = P < vr ? P : vr;
+
   return encode_cache(&p->k, c, c->k, c->k_page_stride, c->k_head_stride, p->k_box) &&
          encode_cache(&p->v, c, c->v, c->v_page_stride, c->v_head_stride, p->v_box) &&
          encode_rows(&p->q, a, a.q, D, a.q_ts, a.q_hs, p->tokens) &&
