@@ -2,15 +2,18 @@
 // the append of a step's keys and values to the paged cache (rnb_rope_append).
 //
 // One pass: a head's row is read once with 16-byte loads (D/8 lanes hold it,
-// so the norm's sum is a few shuffles and the partner of element i, i +- rot/2,
-// is 8 elements in another lane), turned in fp32 and written once, rounded
-// once.  HBM bounds it: 4 (Hq + 2 Hkv) D bytes a token.
+// so the norm's sum is a few shuffles, and the partner of element i, i +- rot/2,
+// is in another lane), turned in fp32 and written once, rounded once.  HBM
+// bounds it: 4 (Hq + 2 Hkv) D bytes a token; what has to be kept small is the
+// instructions a row.  So a group of D/8 lanes stays with one token and walks its
+// heads, four rows under way, with the token's cosines and the norm's weights in
+// registers; the partner comes as raw 16-bit pairs, four shuffles a row.  With
+// few tokens a token's heads are dealt over several groups.
 //
 // Angles: fp32 loses far positions (position 10^5 at frequency 1 is off by
-// 2^-8 rad), so position * frequency and its reduction to half turns are fp64,
-// and sincospif works on the small remainder.  That is rot/2 evaluations a
-// token for all its heads: a CTA computes those of its tokens once into shared
-// memory and serves all heads from there.
+// 2^-8 rad), so position * frequency and its reduction to turns are fp64, and
+// sincospif works on the small remainder.  That is rot/2 evaluations a token for
+// all its heads: the CTA's threads share them through shared memory.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -33,7 +36,8 @@ struct RopeArgs {
   void *q_out, *kc, *vc;
   int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, kc_ps, kc_hs, vc_ps, vc_hs;
   float eps;
-  int T, Hq, Hkv, half, tok, log2p, heads_per_cta;
+  int T, Hq, Hkv, half, log2p;
+  int chunks, heads_a_chunk;  // groups a token, heads each
   int n_axes, interleaved, sec[4];
   uint32_t num_slots;
 };
@@ -50,20 +54,125 @@ __device__ __forceinline__ int axis_of(const RopeArgs& a, int i) {
   return ax;
 }
 
-// Heads are numbered queries first, then keys, then values.  CTA (x, y) takes
-// tokens [x tok, (x + 1) tok) and heads [y heads_per_cta, ...) of each.
+// What a lane keeps over the rows of a token.
+struct Lane {
+  float c[8], s[8];  // cosines and signed sines of its elements (1 and 0 where nothing turns)
+  int partner;       // lane of the warp that holds the partners of its elements
+  bool turned;
+};
+
+// Up to n rows of one token at a stride in elements.
+template <typename T>
+struct Rows {
+  const T* from;
+  int64_t stride;
+  int n;
+  // rows r .. r + 3 (coherent loads: q_out may be q)
+  __device__ __forceinline__ void load(int r, uint4 (&v)[4]) const {
+#pragma unroll
+    for (int y = 0; y < 4; ++y)
+      if (r + y < n) v[y] = __ldcs(reinterpret_cast<const uint4*>(from + (r + y) * stride));
+  }
+};
+
+// The rows of `rows`, turned, to `to`; every lane of the warp calls it with the
+// same n_max >= rows.n, for the shuffles.  `in` holds the first four and, after
+// it, the first four of `next`: four rows are always under way.
+template <typename T, int D>
+__device__ __forceinline__ void turn_rows(uint4 (&in)[4], const Rows<T>& rows, T* to, int64_t to_stride, int n_max,
+                                          const Rows<T>& next, const T* weight, float eps, int e0, int partner_e0,
+                                          const Lane& ln) {
+  constexpr int kLanes = D / 8;
+  float w[8], wp[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = ln.c[i], wp[i] = ln.s[i];
+  if (weight) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(weight + e0));
+    const uint4 b = __ldg(reinterpret_cast<const uint4*>(weight + partner_e0));
+    const uint32_t au[4] = {a.x, a.y, a.z, a.w}, bu[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = Pair<T>::unpack(au[i]), g = Pair<T>::unpack(bu[i]);
+      w[2 * i] *= f.x, w[2 * i + 1] *= f.y, wp[2 * i] *= g.x, wp[2 * i + 1] *= g.y;
+    }
+  }
+  for (int r = 0; r < n_max; r += 4) {
+    uint4 ahead[4] = {};
+    if (r + 4 < n_max)
+      rows.load(r + 4, ahead);
+    else
+      next.load(0, ahead);
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      if (r + y >= n_max) break;
+      const uint32_t u[4] = {in[y].x, in[y].y, in[y].z, in[y].w};
+      float x[8], z[8];
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = Pair<T>::unpack(u[i]);
+        const float2 g = Pair<T>::unpack(__shfl_sync(0xffffffffu, u[i], ln.partner));
+        x[2 * i] = f.x, x[2 * i + 1] = f.y, z[2 * i] = g.x, z[2 * i + 1] = g.y;
+        ss = fmaf(f.x, f.x, fmaf(f.y, f.y, ss));
+      }
+      float sc = 1.f;
+      if (weight) {
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        sc = rsqrtf(fmaf(ss, 1.0f / D, eps));
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = (ln.turned ? x[i] * w[i] + z[i] * wp[i] : x[i] * w[i]) * sc;
+      if (r + y < rows.n)
+        *reinterpret_cast<uint4*>(to + (r + y) * to_stride) = make_uint4(
+            Pair<T>::pack(x[0], x[1]), Pair<T>::pack(x[2], x[3]), Pair<T>::pack(x[4], x[5]), Pair<T>::pack(x[6], x[7]));
+    }
+#pragma unroll
+    for (int y = 0; y < 4; ++y) in[y] = ahead[y];
+  }
+}
+
+// Heads are numbered queries first, then keys, then values; group i of the
+// grid takes heads [c heads_a_chunk, ...) of token i / chunks, c = i % chunks.
 template <typename T, int D>
 __global__ void __launch_bounds__(kRopeThreads) k_rope_append(const RopeArgs a) {
-  constexpr int kLanes = D / 8;                      // lanes holding one head's row
-  constexpr int kGroups = kRopeThreads / kLanes;     // rows in flight in the CTA
-  __shared__ float2 cs[kRopeThreads];                // [tok][half] cos, sin
-  const int tid = threadIdx.x;
-  const int t0 = blockIdx.x * a.tok;
-  const int nt = min(a.tok, a.T - t0);
-  for (int i = tid; i < nt * a.half; i += kRopeThreads) {
-    const int t = i / a.half, f = i - t * a.half;
-    const double p = static_cast<double>(a.pos[static_cast<int64_t>(axis_of(a, f)) * a.T + t0 + t]);
-    // in half turns; the fp64 remainder of whole turns is exact to 2^-52 of the angle
+  constexpr int kLanes = D / 8;                   // lanes holding one head's row
+  constexpr int kGroups = kRopeThreads / kLanes;  // rows in flight in the CTA
+  __shared__ float2 cs[kGroups * D / 2];          // [token][half] cos, sin
+  const int tid = threadIdx.x, lane = tid % kLanes, e0 = lane * 8;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups, all = static_cast<int64_t>(a.T) * a.chunks;
+  const int t_first = static_cast<int>(first / a.chunks);
+  const int t_last = static_cast<int>((min(first + kGroups, all) - 1) / a.chunks);
+
+  // this group's token and heads; its first rows are under way before the angles
+  const int64_t item = first + tid / kLanes;
+  const bool in = item < all;
+  const int t = in ? static_cast<int>(item / a.chunks) : t_first;
+  const int h0 = in ? static_cast<int>(item - static_cast<int64_t>(t) * a.chunks) * a.heads_a_chunk : 0;
+  const int slot = !in ? -1 : a.slots ? a.slots[t] : 0;
+  const int h1 = slot < 0 ? h0 : min(h0 + a.heads_a_chunk, a.Hq + 2 * a.Hkv);  // (no heads: a row left alone)
+  const bool inside = a.slots && static_cast<uint32_t>(slot) < a.num_slots;
+  const int64_t tt = t;
+  const int qb = h0, kb = max(h0 - a.Hq, 0), vb = max(h0 - a.Hq - a.Hkv, 0);
+  const Rows<T> q{static_cast<const T*>(a.q) + tt * a.q_ts + qb * a.q_hs + e0, a.q_hs, max(0, min(h1, a.Hq) - qb)};
+  const Rows<T> k{static_cast<const T*>(a.k) + tt * a.k_ts + kb * a.k_hs + e0, a.k_hs,
+                  inside ? max(0, min(h1 - a.Hq, a.Hkv) - kb) : 0};
+  const Rows<T> v{static_cast<const T*>(a.v) + tt * a.v_ts + vb * a.v_hs + e0, a.v_hs,
+                  inside ? max(0, h1 - a.Hq - a.Hkv - vb) : 0};
+  // a warp's groups run the same number of rounds of each kind
+  const int nq = __reduce_max_sync(0xffffffffu, q.n), nk = __reduce_max_sync(0xffffffffu, k.n);
+  uint4 rows[4] = {};
+  if (nq > 0)
+    q.load(0, rows);
+  else if (nk > 0)
+    k.load(0, rows);
+  else
+    v.load(0, rows);
+
+  for (int i = tid; i < (t_last - t_first + 1) * a.half; i += kRopeThreads) {
+    const int tl = i / a.half, f = i - tl * a.half;
+    const double p = static_cast<double>(a.pos[static_cast<int64_t>(axis_of(a, f)) * a.T + t_first + tl]);
+    // the fp64 remainder of whole turns is exact to 2^-52 of the angle
     double turns = p * static_cast<double>(a.inv_freq[f]) * 0.15915494309189533577;  // 1 / (2 pi)
     turns -= rint(turns);
     float s, c;
@@ -72,82 +181,33 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_append(const RopeArgs a) 
   }
   __syncthreads();
 
-  const int lane = tid % kLanes, e0 = lane * 8;
-  const int heads = a.Hq + 2 * a.Hkv;
-  const int h0 = blockIdx.y * a.heads_per_cta, nh = min(a.heads_per_cta, heads - h0);
-  // a warp's lanes all run the same number of rounds (shuffles below)
-  const int rows = nt * nh;
-  const int rounds = (rows + kGroups - 1) / kGroups;
-  // where this lane's pairs are: the lane that holds elements e0 +- half
   const bool lo = e0 < a.half, turned = e0 < 2 * a.half;
-  const int partner = turned ? (lo ? lane + a.half / 8 : lane - a.half / 8) : lane;
-  const int src = (tid & 31) - lane + partner;
-  for (int r = 0; r < rounds; ++r) {
-    const int row = r * kGroups + tid / kLanes;
-    const bool in = row < rows;
-    const int tl = in ? row / nh : 0, h = h0 + (in ? row - tl * nh : 0), t = t0 + tl;
-    const int slot = a.slots ? a.slots[t] : 0;
-    const bool is_q = h < a.Hq, is_k = !is_q && h < a.Hq + a.Hkv;
-    const int hk = is_q ? h : (h - a.Hq) - (is_k ? 0 : a.Hkv);
-    const T* from = is_q   ? static_cast<const T*>(a.q) + t * a.q_ts + h * a.q_hs
-                    : is_k ? static_cast<const T*>(a.k) + t * a.k_ts + hk * a.k_hs
-                           : static_cast<const T*>(a.v) + t * a.v_ts + hk * a.v_hs;
-    const bool live = in && slot >= 0 && (is_q || static_cast<uint32_t>(slot) < a.num_slots);
-    if (in && slot >= 0 && !is_q && !live && lane == 0) atomicOr(&g_rope_status, RNB_STATUS_BAD_INDEX);
-    uint4 w = make_uint4(0, 0, 0, 0);
-    if (live) w = __ldcs(reinterpret_cast<const uint4*>(from + e0));  // coherent: q_out may be q
-    uint32_t u[4] = {w.x, w.y, w.z, w.w};
-    const T* nw = static_cast<const T*>(is_q ? a.qw : a.kw);
-    const bool is_v = !is_q && !is_k;
-    float x[8];
+  const int pl = turned ? (lo ? lane + a.half / 8 : lane - a.half / 8) : lane;
+  Lane ln;
+  ln.partner = (tid & 31) - lane + pl;
+  ln.turned = turned;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = Pair<T>::unpack(u[i]);
-      x[2 * i] = f.x;
-      x[2 * i + 1] = f.y;
-    }
-    float ss = 0.f;
+  for (int i = 0; i < 8; ++i) {
+    float2 w = make_float2(1.f, 0.f);
+    if (turned) w = cs[(t - t_first) * a.half + (lo ? e0 : e0 - a.half) + i];
+    ln.c[i] = w.x;
+    ln.s[i] = lo ? -w.y : w.y;
+  }
+  if (nq > 0)
+    turn_rows<T, D>(rows, q, static_cast<T*>(a.q_out) + (tt * a.Hq + qb) * D + e0, D, nq, nk > 0 ? k : v,
+                    static_cast<const T*>(a.qw), a.eps, e0, pl * 8, ln);
+  if (!a.slots) return;
+  if (in && slot >= 0 && !inside && lane == 0 && h1 > a.Hq) atomicOr(&g_rope_status, RNB_STATUS_BAD_INDEX);
+  const int64_t page = inside ? slot >> a.log2p : 0, off = inside ? (slot & ((1 << a.log2p) - 1)) * D : 0;
+  if (nk > 0)
+    turn_rows<T, D>(rows, k, static_cast<T*>(a.kc) + page * a.kc_ps + kb * a.kc_hs + off + e0, a.kc_hs, nk, v,
+                    static_cast<const T*>(a.kw), a.eps, e0, pl * 8, ln);
+  T* to = static_cast<T*>(a.vc) + page * a.vc_ps + vb * a.vc_hs + off + e0;
+  for (int r = 0; r < v.n; r += 4) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (nw && !is_v) {
-      const float sc = 1.0f / sqrtf(ss * (1.0f / D) + a.eps);
-      const uint4 g = __ldg(reinterpret_cast<const uint4*>(nw + e0));
-      const uint32_t gu[4] = {g.x, g.y, g.z, g.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = Pair<T>::unpack(gu[i]);
-        x[2 * i] *= sc * f.x;
-        x[2 * i + 1] *= sc * f.y;
-      }
-    }
-    float y[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], src);
-    if (!is_v && turned) {
-      const float2* c = cs + tl * a.half + (lo ? e0 : e0 - a.half);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 v = c[i];
-        x[i] = lo ? x[i] * v.x - y[i] * v.y : x[i] * v.x + y[i] * v.y;
-      }
-    }
-    if (live) {
-      uint4 o = w;
-      if (!is_v)
-        o = make_uint4(Pair<T>::pack(x[0], x[1]), Pair<T>::pack(x[2], x[3]), Pair<T>::pack(x[4], x[5]),
-                       Pair<T>::pack(x[6], x[7]));
-      T* to;
-      if (is_q) {
-        to = static_cast<T*>(a.q_out) + (static_cast<int64_t>(t) * a.Hq + h) * D;
-      } else {
-        const int64_t page = slot >> a.log2p, off = (slot & ((1 << a.log2p) - 1)) * D;
-        to = is_k ? static_cast<T*>(a.kc) + page * a.kc_ps + hk * a.kc_hs + off
-                  : static_cast<T*>(a.vc) + page * a.vc_ps + hk * a.vc_hs + off;
-      }
-      *reinterpret_cast<uint4*>(to + e0) = o;
-    }
+    for (int y = 0; y < 4; ++y)
+      if (r + y < v.n) *reinterpret_cast<uint4*>(to + (r + y) * a.vc_hs) = rows[y];
+    v.load(r + 4, rows);
   }
 }
 
@@ -180,7 +240,9 @@ int check_rope(const rnb_rope_desc* d) {
 }
 
 template <typename T>
-void launch_rope(const RopeArgs& a, int D, dim3 grid, cudaStream_t st) {
+void launch_rope(const RopeArgs& a, int D, int64_t groups, cudaStream_t st) {
+  const int a_cta = kRopeThreads / (D / 8);
+  const unsigned grid = static_cast<unsigned>((groups + a_cta - 1) / a_cta);
   if (D == 64)
     k_rope_append<T, 64><<<grid, kRopeThreads, 0, st>>>(a);
   else if (D == 128)
@@ -241,22 +303,20 @@ extern "C" int rnb_rope_append(const rnb_rope_desc* d, const void* q, const void
   a.n_axes = d->n_axes, a.interleaved = d->interleaved;
   for (int i = 0; i < 4; ++i) a.sec[i] = d->sections[i];
 
-  // Many tokens: as many a CTA as give each thread one angle, all heads from
-  // them.  Few: one token a CTA, its heads dealt over CTAs until the SMs are
-  // covered (each repeats the token's angles, rot/2 of them).
-  const int heads = a.Hq + 2 * a.Hkv, sms = dev_info().sms;
-  const int groups = kRopeThreads / static_cast<int>(D / 8);
-  int tok = kRopeThreads / a.half;
-  while (tok > 1 && (a.T + tok - 1) / tok < 2 * sms) tok /= 2;
-  a.tok = tok;
-  const int ctas = (a.T + tok - 1) / tok;
-  int split = 1;
-  while (split < heads && ctas * split < sms && (heads + split - 1) / split > groups) ++split;
-  a.heads_per_cta = (heads + split - 1) / split;
-  const dim3 grid(ctas, (heads + a.heads_per_cta - 1) / a.heads_per_cta);
+  // Many tokens: a group a token.  Few: a token's heads over as many groups as
+  // cover the SMs with four rows a group or more.
+  const int heads = a.Hq + 2 * a.Hkv;
+  const int64_t want = static_cast<int64_t>(dev_info().sms) * (kRopeThreads / static_cast<int>(D / 8));
+  int64_t chunks = (want + a.T - 1) / a.T;
+  const int64_t most = (heads + 3) / 4;
+  if (chunks > most) chunks = most;
+  a.heads_a_chunk = static_cast<int>((heads + chunks - 1) / chunks);
+  a.chunks = (heads + a.heads_a_chunk - 1) / a.heads_a_chunk;
+  const int64_t groups = static_cast<int64_t>(a.T) * a.chunks;
+  if (groups > INT32_MAX) return fail(RNB_ERR_INVALID, "rnb_rope_append: too many rows");
   if (d->dtype == RNB_DTYPE_BF16)
-    launch_rope<__nv_bfloat16>(a, static_cast<int>(D), grid, static_cast<cudaStream_t>(stream));
+    launch_rope<__nv_bfloat16>(a, static_cast<int>(D), groups, static_cast<cudaStream_t>(stream));
   else
-    launch_rope<__half>(a, static_cast<int>(D), grid, static_cast<cudaStream_t>(stream));
+    launch_rope<__half>(a, static_cast<int>(D), groups, static_cast<cudaStream_t>(stream));
   return launch_status("rnb_rope_append");
 }
