@@ -54,11 +54,12 @@ __device__ __forceinline__ int axis_of(const RopeArgs& a, int i) {
   return ax;
 }
 
-// What a lane keeps over the rows of a token.
+// Where a lane's elements and their partners are.
 struct Lane {
-  float c[8], s[8];  // cosines and signed sines of its elements (1 and 0 where nothing turns)
-  int partner;       // lane of the warp that holds the partners of its elements
-  bool turned;
+  const float2* cs;  // cosine and sine of its 8 pairs (only where they turn)
+  int e0, partner_e0;  // first elements, its own and its partner's
+  int partner;         // the partner's lane in the warp
+  bool turned, lo;     // its elements turn; they are the pairs' first elements
 };
 
 // Up to n rows of one token at a stride in elements.
@@ -80,21 +81,23 @@ struct Rows {
 // it, the first four of `next`: four rows are always under way.
 template <typename T, int D>
 __device__ __forceinline__ void turn_rows(uint4 (&in)[4], const Rows<T>& rows, T* to, int64_t to_stride, int n_max,
-                                          const Rows<T>& next, const T* weight, float eps, int e0, int partner_e0,
-                                          const Lane& ln) {
+                                          const Rows<T>& next, const T* weight, float eps, const Lane& ln) {
   constexpr int kLanes = D / 8;
-  float w[8], wp[8];
+  // y = x w + z wp with z the partners: cosines and signed sines, times the norm's weights
+  float2 w[4], wp[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i] = ln.c[i], wp[i] = ln.s[i];
+  for (int i = 0; i < 4; ++i) {
+    float4 c = make_float4(1.f, 0.f, 1.f, 0.f);
+    if (ln.turned) c = *reinterpret_cast<const float4*>(ln.cs + 2 * i);
+    w[i] = make_float2(c.x, c.z);
+    wp[i] = ln.lo ? make_float2(-c.y, -c.w) : make_float2(c.y, c.w);
+  }
   if (weight) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(weight + e0));
-    const uint4 b = __ldg(reinterpret_cast<const uint4*>(weight + partner_e0));
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(weight + ln.e0));
+    const uint4 b = __ldg(reinterpret_cast<const uint4*>(weight + ln.partner_e0));
     const uint32_t au[4] = {a.x, a.y, a.z, a.w}, bu[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = Pair<T>::unpack(au[i]), g = Pair<T>::unpack(bu[i]);
-      w[2 * i] *= f.x, w[2 * i + 1] *= f.y, wp[2 * i] *= g.x, wp[2 * i + 1] *= g.y;
-    }
+    for (int i = 0; i < 4; ++i) w[i] = mul2(w[i], Pair<T>::unpack(au[i])), wp[i] = mul2(wp[i], Pair<T>::unpack(bu[i]));
   }
   for (int r = 0; r < n_max; r += 4) {
     uint4 ahead[4] = {};
@@ -106,26 +109,27 @@ __device__ __forceinline__ void turn_rows(uint4 (&in)[4], const Rows<T>& rows, T
     for (int y = 0; y < 4; ++y) {
       if (r + y >= n_max) break;
       const uint32_t u[4] = {in[y].x, in[y].y, in[y].z, in[y].w};
-      float x[8], z[8];
-      float ss = 0.f;
+      float2 x[4];
+      float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
+        const uint32_t z = __shfl_sync(0xffffffffu, u[i], ln.partner);
         const float2 f = Pair<T>::unpack(u[i]);
-        const float2 g = Pair<T>::unpack(__shfl_sync(0xffffffffu, u[i], ln.partner));
-        x[2 * i] = f.x, x[2 * i + 1] = f.y, z[2 * i] = g.x, z[2 * i + 1] = g.y;
-        ss = fmaf(f.x, f.x, fmaf(f.y, f.y, ss));
+        ss = fma2(f, f, ss);
+        x[i] = fma2(Pair<T>::unpack(ln.turned ? z : 0u), wp[i], mul2(f, w[i]));  // (0: what does not turn passes any bits)
       }
-      float sc = 1.f;
       if (weight) {
+        float sum = ss.x + ss.y;
 #pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        sc = rsqrtf(fmaf(ss, 1.0f / D, eps));
+        for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const float sc = rsqrtf(fmaf(sum, 1.0f / D, eps));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = mul2(x[i], make_float2(sc, sc));
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = (ln.turned ? x[i] * w[i] + z[i] * wp[i] : x[i] * w[i]) * sc;
       if (r + y < rows.n)
-        *reinterpret_cast<uint4*>(to + (r + y) * to_stride) = make_uint4(
-            Pair<T>::pack(x[0], x[1]), Pair<T>::pack(x[2], x[3]), Pair<T>::pack(x[4], x[5]), Pair<T>::pack(x[6], x[7]));
+        *reinterpret_cast<uint4*>(to + (r + y) * to_stride) =
+            make_uint4(Pair<T>::pack(x[0].x, x[0].y), Pair<T>::pack(x[1].x, x[1].y), Pair<T>::pack(x[2].x, x[2].y),
+                       Pair<T>::pack(x[3].x, x[3].y));
     }
 #pragma unroll
     for (int y = 0; y < 4; ++y) in[y] = ahead[y];
@@ -135,10 +139,10 @@ __device__ __forceinline__ void turn_rows(uint4 (&in)[4], const Rows<T>& rows, T
 // Heads are numbered queries first, then keys, then values; group i of the
 // grid takes heads [c heads_a_chunk, ...) of token i / chunks, c = i % chunks.
 template <typename T, int D>
-__global__ void __launch_bounds__(kRopeThreads) k_rope_append(const RopeArgs a) {
+__global__ void __launch_bounds__(kRopeThreads, 3) k_rope_append(const RopeArgs a) {
   constexpr int kLanes = D / 8;                   // lanes holding one head's row
   constexpr int kGroups = kRopeThreads / kLanes;  // rows in flight in the CTA
-  __shared__ float2 cs[kGroups * D / 2];          // [token][half] cos, sin
+  __shared__ __align__(16) float2 cs[kGroups * D / 2];  // [token][half] cos, sin
   const int tid = threadIdx.x, lane = tid % kLanes, e0 = lane * 8;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups, all = static_cast<int64_t>(a.T) * a.chunks;
   const int t_first = static_cast<int>(first / a.chunks);
@@ -181,27 +185,20 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope_append(const RopeArgs a) 
   }
   __syncthreads();
 
-  const bool lo = e0 < a.half, turned = e0 < 2 * a.half;
-  const int pl = turned ? (lo ? lane + a.half / 8 : lane - a.half / 8) : lane;
   Lane ln;
-  ln.partner = (tid & 31) - lane + pl;
-  ln.turned = turned;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float2 w = make_float2(1.f, 0.f);
-    if (turned) w = cs[(t - t_first) * a.half + (lo ? e0 : e0 - a.half) + i];
-    ln.c[i] = w.x;
-    ln.s[i] = lo ? -w.y : w.y;
-  }
+  ln.e0 = e0, ln.lo = e0 < a.half, ln.turned = e0 < 2 * a.half;
+  const int pl = ln.turned ? (ln.lo ? lane + a.half / 8 : lane - a.half / 8) : lane;
+  ln.partner = (tid & 31) - lane + pl, ln.partner_e0 = pl * 8;
+  ln.cs = cs + (t - t_first) * a.half + (ln.turned ? (ln.lo ? e0 : e0 - a.half) : 0);
   if (nq > 0)
     turn_rows<T, D>(rows, q, static_cast<T*>(a.q_out) + (tt * a.Hq + qb) * D + e0, D, nq, nk > 0 ? k : v,
-                    static_cast<const T*>(a.qw), a.eps, e0, pl * 8, ln);
+                    static_cast<const T*>(a.qw), a.eps, ln);
   if (!a.slots) return;
   if (in && slot >= 0 && !inside && lane == 0 && h1 > a.Hq) atomicOr(&g_rope_status, RNB_STATUS_BAD_INDEX);
   const int64_t page = inside ? slot >> a.log2p : 0, off = inside ? (slot & ((1 << a.log2p) - 1)) * D : 0;
   if (nk > 0)
     turn_rows<T, D>(rows, k, static_cast<T*>(a.kc) + page * a.kc_ps + kb * a.kc_hs + off + e0, a.kc_hs, nk, v,
-                    static_cast<const T*>(a.kw), a.eps, e0, pl * 8, ln);
+                    static_cast<const T*>(a.kw), a.eps, ln);
   T* to = static_cast<T*>(a.vc) + page * a.vc_ps + vb * a.vc_hs + off + e0;
   for (int r = 0; r < v.n; r += 4) {
 #pragma unroll
