@@ -24,7 +24,8 @@
 namespace rnb {
 namespace {
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 64;  // small CTAs: no SM is left with the last large one
+constexpr int kRopeCtas = 12;     // resident on an SM
 
 __device__ uint32_t g_rope_status;
 
@@ -37,7 +38,7 @@ struct RopeArgs {
   int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, kc_ps, kc_hs, vc_ps, vc_hs;
   float eps;
   int T, Hq, Hkv, half, log2p;
-  int chunks, heads_a_chunk;  // groups a token, heads each
+  int heads_a_chunk;
   int n_axes, interleaved, sec[4];
   uint32_t num_slots;
 };
@@ -136,23 +137,20 @@ __device__ __forceinline__ void turn_rows(uint4 (&in)[4], const Rows<T>& rows, T
   }
 }
 
-// Heads are numbered queries first, then keys, then values; group i of the
-// grid takes heads [c heads_a_chunk, ...) of token i / chunks, c = i % chunks.
+// Heads are numbered queries first, then keys, then values; the groups of CTA
+// (x, y) take heads [y heads_a_chunk, ...) of a token each.  (Groups of a warp
+// have the same heads: a warp walks as many as its longest group.)
 template <typename T, int D>
-__global__ void __launch_bounds__(kRopeThreads, 3) k_rope_append(const RopeArgs a) {
+__global__ void __launch_bounds__(kRopeThreads, kRopeCtas) k_rope_append(const RopeArgs a) {
   constexpr int kLanes = D / 8;                   // lanes holding one head's row
   constexpr int kGroups = kRopeThreads / kLanes;  // rows in flight in the CTA
   __shared__ __align__(16) float2 cs[kGroups * D / 2];  // [token][half] cos, sin
   const int tid = threadIdx.x, lane = tid % kLanes, e0 = lane * 8;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups, all = static_cast<int64_t>(a.T) * a.chunks;
-  const int t_first = static_cast<int>(first / a.chunks);
-  const int t_last = static_cast<int>((min(first + kGroups, all) - 1) / a.chunks);
+  const int t_first = blockIdx.x * kGroups, t_last = min(t_first + kGroups, a.T) - 1;
 
   // this group's token and heads; its first rows are under way before the angles
-  const int64_t item = first + tid / kLanes;
-  const bool in = item < all;
-  const int t = in ? static_cast<int>(item / a.chunks) : t_first;
-  const int h0 = in ? static_cast<int>(item - static_cast<int64_t>(t) * a.chunks) * a.heads_a_chunk : 0;
+  const bool in = t_first + tid / kLanes < a.T;
+  const int t = in ? t_first + tid / kLanes : t_first, h0 = blockIdx.y * a.heads_a_chunk;
   const int slot = !in ? -1 : a.slots ? a.slots[t] : 0;
   const int h1 = slot < 0 ? h0 : min(h0 + a.heads_a_chunk, a.Hq + 2 * a.Hkv);  // (no heads: a row left alone)
   const bool inside = a.slots && static_cast<uint32_t>(slot) < a.num_slots;
@@ -237,9 +235,7 @@ int check_rope(const rnb_rope_desc* d) {
 }
 
 template <typename T>
-void launch_rope(const RopeArgs& a, int D, int64_t groups, cudaStream_t st) {
-  const int a_cta = kRopeThreads / (D / 8);
-  const unsigned grid = static_cast<unsigned>((groups + a_cta - 1) / a_cta);
+void launch_rope(const RopeArgs& a, int D, dim3 grid, cudaStream_t st) {
   if (D == 64)
     k_rope_append<T, 64><<<grid, kRopeThreads, 0, st>>>(a);
   else if (D == 128)
@@ -301,19 +297,18 @@ extern "C" int rnb_rope_append(const rnb_rope_desc* d, const void* q, const void
   for (int i = 0; i < 4; ++i) a.sec[i] = d->sections[i];
 
   // Many tokens: a group a token.  Few: a token's heads over as many groups as
-  // cover the SMs with four rows a group or more.
-  const int heads = a.Hq + 2 * a.Hkv;
-  const int64_t want = static_cast<int64_t>(dev_info().sms) * (kRopeThreads / static_cast<int>(D / 8));
-  int64_t chunks = (want + a.T - 1) / a.T;
-  const int64_t most = (heads + 3) / 4;
-  if (chunks > most) chunks = most;
+  // the SMs hold at once, four rows a group or more.
+  const int heads = a.Hq + 2 * a.Hkv, groups = kRopeThreads / static_cast<int>(D / 8);
+  const int64_t hold = static_cast<int64_t>(dev_info().sms) * kRopeCtas * groups;
+  int64_t chunks = hold / a.T;  // (rounded up, 4097 tokens of 48 heads took 27 us instead of 25)
+  if (chunks < 1) chunks = 1;
+  if (chunks > (heads + 3) / 4) chunks = (heads + 3) / 4;
   a.heads_a_chunk = static_cast<int>((heads + chunks - 1) / chunks);
-  a.chunks = (heads + a.heads_a_chunk - 1) / a.heads_a_chunk;
-  const int64_t groups = static_cast<int64_t>(a.T) * a.chunks;
-  if (groups > INT32_MAX) return fail(RNB_ERR_INVALID, "rnb_rope_append: too many rows");
+  const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(a.T) + groups - 1) / groups),
+                  static_cast<unsigned>((heads + a.heads_a_chunk - 1) / a.heads_a_chunk));
   if (d->dtype == RNB_DTYPE_BF16)
-    launch_rope<__nv_bfloat16>(a, static_cast<int>(D), groups, static_cast<cudaStream_t>(stream));
+    launch_rope<__nv_bfloat16>(a, static_cast<int>(D), grid, static_cast<cudaStream_t>(stream));
   else
-    launch_rope<__half>(a, static_cast<int>(D), groups, static_cast<cudaStream_t>(stream));
+    launch_rope<__half>(a, static_cast<int>(D), grid, static_cast<cudaStream_t>(stream));
   return launch_status("rnb_rope_append");
 }
