@@ -109,38 +109,53 @@ struct Begun {
   int q0, work, h, tile;
 };
 
+// A tile's part that one CTA covers: units [blk, blk + n) of the tile's nblk.
+struct Segment {
+  int b, q0, rows, len, blk0, nblk;  // its request
+  int h, tile, blk, n;               // n 0: none
+};
+
 template <typename T, int D, int NT>
 struct __align__(16) Smem {
   float m[kWarps][8 * NT], l[kWarps][8 * NT];
   float o[kWarps][8 * NT][D + 4];
+  T q[2][8 * NT][D + 32];  // queries of this segment and the next; rows 64 bytes off in the banks
+  Segment seg[3];          // this one and the two behind it
 };
 
-// What a warp loads for one step: NS subtiles of 16 positions.
+// What a warp loads for one step: NS subtiles of 16 positions, 64 registers of K
+// and 64 of V a lane (half as many where 16 rows leave no more).
 template <int D, int NT>
 struct Steps {
-  static constexpr int NS = NT == 1 ? 256 / D : (D == 64 ? 2 : 1);
+  static constexpr int NS = D == 64 && NT == 2 ? 2 : 256 / D;
 };
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
   constexpr int R = 8 * NT, NS = Steps<D, NT>::NS, KC = D / 32, VC = D / 64;
+  constexpr int kStep = 16 * NS, kStride = kWarps * kStep;
+  constexpr int kTile = 512 / D;  // what starting and joining a tile costs, in units (without it
+  // ragged batches left half of the SMs idle: 204 instead of 117 us, 63 instead of 35)
   __shared__ Smem<T, D, NT> sm;
-  __shared__ int64_t wsum[kWarps], start_rem, total;
-  __shared__ int start_b;
+  __shared__ int64_t wsum[kWarps], total;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   Begun* begun = reinterpret_cast<Begun*>(a.ws);
   if (tid == 0) begun[blockIdx.x].last = -1;
 
-  // ---- this CTA's share
+  // ---- this CTA's share.  The thread whose requests hold its first unit deals the
+  // segments from there, two ahead of the one in work: it stands at cost p_at of row
+  // tile tile_at of key head h_at of request `at`, whose numbers are c0, c1, len.
+  bool dealer = false;
+  int64_t start_rem = 0;
+  int at = 0, h_at = 0, tile_at = 0, p_at = 0, c0 = 0, c1 = 0, len = 0;
   {
     const int per = (a.B + kThreads - 1) / kThreads;
     const int lo = min(tid * per, a.B), hi = min(lo + per, a.B);
     auto units = [&](int b) {
-      int c0, c1, len;
       read_request(a, b, c0, c1, len);
       if (blockIdx.x == 0 && (len < 0 || len > a.max_kv)) atomicOr(&g_attn_status, RNB_STATUS_BAD_INDEX);
       const Request r = request_of<R>(a, c0, c1, len);
-      return static_cast<int64_t>(r.ntile) * r.nblk * a.Hkv;
+      return static_cast<int64_t>(r.ntile) * (r.nblk + kTile) * a.Hkv;
     };
     int64_t sum = 0;
     for (int b = lo; b < hi; ++b) sum += units(b);
@@ -158,68 +173,161 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
     __syncthreads();
     const int64_t share = (total + gridDim.x - 1) / gridDim.x, u0 = share * blockIdx.x;
     if (u0 >= base && u0 < base + sum) {
-      int64_t rem = u0 - base;
-      int b = lo;
-      for (int64_t n = units(b); rem >= n; n = units(b)) {
-        rem -= n;
-        ++b;
+      dealer = true;
+      start_rem = u0 - base;
+      at = lo;
+      for (int64_t n = per == 1 ? sum : units(at); start_rem >= n && at + 1 < hi; n = units(at)) {
+        start_rem -= n;
+        ++at;
       }
-      start_b = b;
-      start_rem = rem;
     }
-    __syncthreads();
   }
   const int64_t share = (total + gridDim.x - 1) / gridDim.x, u0 = share * blockIdx.x;
   const int64_t u1 = min(u0 + share, total);
   if (u0 >= u1) return;
-  int b = start_b;
-  int64_t rem = start_rem;
-  int c0, c1, len;
-  read_request(a, b, c0, c1, len);
-  Request rq = request_of<R>(a, c0, c1, len);
-  read_request(a, b + 1, c0, c1, len);  // one ahead
 
-  for (int64_t u = u0; u < u1;) {
-    const int64_t mine = static_cast<int64_t>(rq.ntile) * rq.nblk * a.Hkv;
-    if (rem >= mine) {
-      rem -= mine;
-      ++b;
-      rq = request_of<R>(a, c0, c1, len);
-      read_request(a, b + 1, c0, c1, len);
-      continue;
+  int64_t u_at = u0;
+  auto deal = [&](Segment& sg) {
+    sg.n = 0;
+    while (u_at < u1 && at < a.B) {  // (the second: lengths that change under way must not hang it)
+      const Request rq = request_of<R>(a, c0, c1, len);
+      if (h_at < a.Hkv && rq.ntile > 0) {
+        const int cost = kTile + rq.nblk;
+        const int take = static_cast<int>(min(static_cast<int64_t>(cost - p_at), u1 - u_at));
+        const int first = max(p_at - kTile, 0), end = max(p_at + take - kTile, 0);
+        sg.b = at, sg.q0 = rq.q0, sg.rows = rq.rows, sg.len = rq.len, sg.blk0 = rq.blk0, sg.nblk = rq.nblk;
+        sg.h = h_at, sg.tile = tile_at, sg.blk = first, sg.n = end - first;
+        u_at += take;
+        p_at += take;
+        if (p_at == cost) {
+          p_at = 0;
+          if (++tile_at == rq.ntile) tile_at = 0, ++h_at;
+        }
+      }
+      if (h_at == a.Hkv || rq.ntile == 0) {  // the next request's numbers are on their way when they are asked for
+        h_at = tile_at = p_at = 0;
+        read_request(a, ++at, c0, c1, len);
+      }
+      if (sg.n > 0) return;
     }
-    const int tile_of = static_cast<int>(rem / rq.nblk), blk = static_cast<int>(rem - static_cast<int64_t>(tile_of) * rq.nblk);
-    const int h = tile_of / rq.ntile, tile = tile_of - h * rq.ntile;
-    const int n = static_cast<int>(min(static_cast<int64_t>(rq.nblk - blk), u1 - u));
-    const int work = rq.rows * a.group;
+  };
+  if (dealer) {
+    const Request rq = request_of<R>(a, c0, c1, len);
+    const int cost = rq.nblk + kTile;
+    const int64_t tile_of = start_rem < INT_MAX ? static_cast<int>(start_rem) / cost : start_rem / cost;
+    p_at = static_cast<int>(start_rem - tile_of * cost);
+    h_at = static_cast<int>(tile_of / max(rq.ntile, 1));
+    tile_at = static_cast<int>(tile_of - static_cast<int64_t>(h_at) * rq.ntile);
+    deal(sm.seg[0]);
+    deal(sm.seg[1]);
+  }
+  __syncthreads();
 
-    // ---- the tile's queries, in K's element order, and each row's positions
-    uint32_t qf[NT][KC][4];
+  // ---- what a warp's loads go by
+  const T *kh = nullptr, *vh = nullptr;
+  const int32_t* row_table = nullptr;
+  int s = 0, s_end = 0;  // positions: the step whose K and V are (being) loaded, the segment's end
+  const int pmask = (1 << a.log2p) - 1;
+  auto positions_end = [&](const Segment& sg) {
+    const int last = sg.len - sg.rows + min(sg.tile * R + R - 1, sg.rows * a.group - 1) / a.group;
+    return min((sg.blk0 + sg.blk + sg.n) * kUnit, last + 1);
+  };
+  auto enter = [&](const Segment& sg) {
+    s = s_end = 0;
+    if (sg.n > 0) {
+      kh = static_cast<const T*>(a.kc) + sg.h * a.kc_hs + g * D + 8 * c;
+      vh = static_cast<const T*>(a.vc) + sg.h * a.vc_hs + 2 * c * D + 8 * g;
+      row_table = a.table + static_cast<int64_t>(sg.b) * a.W;
+      s = (sg.blk0 + sg.blk) * kUnit + warp * kStep;
+      s_end = positions_end(sg);
+    }
+  };
+  auto pages_of = [&](const int32_t* tab, int from, int end, int (&pid)[NS]) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int row = tile * R + nt * 8 + g, i = row / a.group, j = row - i * a.group;
-      const T* qp = static_cast<const T*>(a.q) + (rq.q0 + i) * a.q_ts + (h * a.group + j) * a.q_hs + 8 * c;
+    for (int ns = 0; ns < NS; ++ns) {
+      const int st = from + 16 * ns;
+      pid[ns] = st < end ? __ldg(tab + (st >> a.log2p)) : -1;
+    }
+  };
+  uint4 kr[NS][KC][2], vr[NS][VC][4];
+  auto load_k = [&](const int (&pid)[NS]) {
 #pragma unroll
-      for (int s = 0; s < KC; ++s) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (row < work) v = __ldg(reinterpret_cast<const uint4*>(qp + 32 * s));
-        qf[nt][s][0] = v.x, qf[nt][s][1] = v.y, qf[nt][s][2] = v.z, qf[nt][s][3] = v.w;
+    for (int ns = 0; ns < NS; ++ns) {
+      const bool ok = static_cast<uint32_t>(pid[ns]) < static_cast<uint32_t>(a.num_pages);
+      const T* p = kh + (ok ? pid[ns] : 0) * a.kc_ps + ((s + 16 * ns) & pmask) * D;
+#pragma unroll
+      for (int i = 0; i < KC; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          kr[ns][i][e] = make_uint4(0, 0, 0, 0);
+          if (ok) kr[ns][i][e] = ld_stream_v4(p + 32 * i + 8 * e * D);
+        }
+    }
+  };
+  auto load_v = [&](const int (&pid)[NS]) {
+#pragma unroll
+    for (int ns = 0; ns < NS; ++ns) {
+      const bool ok = static_cast<uint32_t>(pid[ns]) < static_cast<uint32_t>(a.num_pages);
+      const T* p = vh + (ok ? pid[ns] : 0) * a.vc_ps + ((s + 16 * ns) & pmask) * D;
+#pragma unroll
+      for (int i = 0; i < VC; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          vr[ns][i][e] = make_uint4(0, 0, 0, 0);
+          if (ok) vr[ns][i][e] = ld_stream_v4(p + 64 * i + ((e & 1) + 8 * (e >> 1)) * D);
+        }
+    }
+  };
+  auto load_q = [&](const Segment& sg, int buf) {
+    constexpr int kPer = D / 8;
+    for (int x = tid; x < R * kPer; x += kThreads) {
+      const int r = x / kPer, e = (x - r * kPer) * 8, row = sg.tile * R + r, i = row / a.group, j = row - i * a.group;
+      if (row < sg.rows * a.group)
+        cp_async16(&sm.q[buf][r][e],
+                   static_cast<const T*>(a.q) + (sg.q0 + i) * a.q_ts + (sg.h * a.group + j) * a.q_hs + e);
+      else
+        *reinterpret_cast<uint4*>(&sm.q[buf][r][e]) = make_uint4(0, 0, 0, 0);
+    }
+  };
+
+  int pid[NS], nxt[NS], first_pid[NS];
+  load_q(sm.seg[0], 0);
+  enter(sm.seg[0]);
+  pages_of(row_table, s, s_end, pid);
+  load_k(pid);
+  load_v(pid);
+  pages_of(row_table, s + kStride, s_end, nxt);
+  cp_async_wait_all();
+  __syncthreads();
+
+  for (int x = 0;; ++x) {
+    const Segment sg = sm.seg[x % 3];
+    if (sg.n == 0) break;
+    const int work = sg.rows * a.group, row0 = sg.tile * R, seg_end = s_end;
+    {
+      // the next segment: its queries, and the pages of this warp's first step in it
+      const Segment& ns = sm.seg[(x + 1) % 3];
+#pragma unroll
+      for (int y = 0; y < NS; ++y) first_pid[y] = -1;
+      if (ns.n > 0) {
+        load_q(ns, (x + 1) & 1);
+        pages_of(a.table + static_cast<int64_t>(ns.b) * a.W, (ns.blk0 + ns.blk) * kUnit + warp * kStep,
+                 positions_end(ns), first_pid);
       }
     }
-    const int p0 = rq.len - rq.rows;  // position of the request's first row
+    const int p0 = sg.len - sg.rows;  // position of the request's first row
     int seen_hi[NT][2], seen_lo[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int row = min(tile * R + nt * 8 + 2 * c + e, work - 1), p = p0 + row / a.group;
+        const int row = min(row0 + nt * 8 + 2 * c + e, work - 1), p = p0 + row / a.group;
         seen_hi[nt][e] = p;
         seen_lo[nt][e] = a.window > 0 ? p - a.window + 1 : INT_MIN;
       }
-    const int first_p = p0 + (tile * R) / a.group, last_p = p0 + min(tile * R + R - 1, work - 1) / a.group;
-    const int all_lo = a.window > 0 ? last_p - a.window + 1 : INT_MIN;    // from here every row sees, up to first_p
-    const int any_lo = a.window > 0 ? first_p - a.window + 1 : INT_MIN;   // before here none does
-    const int s_end = min((rq.blk0 + blk + n) * kUnit, last_p + 1);
+    const int first_p = p0 + row0 / a.group, last_p = p0 + min(row0 + R - 1, work - 1) / a.group;
+    const int all_lo = a.window > 0 ? last_p - a.window + 1 : INT_MIN;   // from here every row sees, up to first_p
+    const int any_lo = a.window > 0 ? first_p - a.window + 1 : INT_MIN;  // before here none does
 
     float o[NT][VC][4][4];
     float m[NT][2], l[NT][2];
@@ -228,107 +336,85 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) m[nt][e] = -INFINITY, l[nt][e] = 0.f;
 #pragma unroll
-      for (int s = 0; s < VC; ++s)
+      for (int i = 0; i < VC; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[nt][s][j][e] = 0.f;
+          for (int e = 0; e < 4; ++e) o[nt][i][j][e] = 0.f;
     }
 
-    const int32_t* row_table = a.table + static_cast<int64_t>(b) * a.W;
-    const T* kh = static_cast<const T*>(a.kc) + h * a.kc_hs + g * D + 8 * c;
-    const T* vh = static_cast<const T*>(a.vc) + h * a.vc_hs + 2 * c * D + 8 * g;
-    const int pmask = (1 << a.log2p) - 1;
-    auto pages_of = [&](int s, int (&pid)[NS]) {
+    bool more = s < seg_end;
+    bool entered = false;  // the loads are at the next segment
+    auto advance = [&]() {  // to the next step, here or in the next segment
+      s += kStride;
+      more = s < seg_end;
+      if (more) {
 #pragma unroll
-      for (int ns = 0; ns < NS; ++ns) {
-        const int st = s + 16 * ns;
-        pid[ns] = st < s_end ? __ldg(row_table + (st >> a.log2p)) : -1;
+        for (int y = 0; y < NS; ++y) pid[y] = nxt[y];
+      } else {
+        enter(sm.seg[(x + 1) % 3]);
+        entered = true;
+#pragma unroll
+        for (int y = 0; y < NS; ++y) pid[y] = first_pid[y];
       }
     };
-    uint4 kr[NS][KC][2], vr[NS][VC][4];
-    auto load_k = [&](int s, const int (&pid)[NS]) {
-#pragma unroll
-      for (int ns = 0; ns < NS; ++ns) {
-        const bool ok = static_cast<uint32_t>(pid[ns]) < static_cast<uint32_t>(a.num_pages);
-        const T* p = kh + (ok ? pid[ns] : 0) * a.kc_ps + ((s + 16 * ns) & pmask) * D;
-#pragma unroll
-        for (int i = 0; i < KC; ++i)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            kr[ns][i][e] = make_uint4(0, 0, 0, 0);
-            if (ok) kr[ns][i][e] = ld_stream_v4(p + 32 * i + 8 * e * D);
-          }
-      }
-    };
-    auto load_v = [&](int s, const int (&pid)[NS]) {
-#pragma unroll
-      for (int ns = 0; ns < NS; ++ns) {
-        const bool ok = static_cast<uint32_t>(pid[ns]) < static_cast<uint32_t>(a.num_pages);
-        const T* p = vh + (ok ? pid[ns] : 0) * a.vc_ps + ((s + 16 * ns) & pmask) * D;
-#pragma unroll
-        for (int i = 0; i < VC; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            vr[ns][i][e] = make_uint4(0, 0, 0, 0);
-            if (ok) vr[ns][i][e] = ld_stream_v4(p + 64 * i + ((e & 1) + 8 * (e >> 1)) * D);
-          }
-      }
-    };
-
-    constexpr int kStep = 16 * NS;
-    int s = (rq.blk0 + blk) * kUnit + warp * kStep;
-    int pid[NS], nxt[NS];
-    pages_of(s, pid);
-    load_k(s, pid);
-    load_v(s, pid);
-    pages_of(s + kWarps * kStep, nxt);
-    for (; s < s_end; s += kWarps * kStep) {
+    while (more) {
       // S^T
-      float sc[NS][NT][4];
+      float sc[NS][NT][4], sd[NS][NT][4];  // two chains of products
 #pragma unroll
       for (int ns = 0; ns < NS; ++ns)
 #pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[ns][nt][e] = sd[ns][nt][e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < KC; ++i)
+#pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
+          const uint4 qf = *reinterpret_cast<const uint4*>(&sm.q[x & 1][nt * 8 + g][32 * i + 8 * c]);
 #pragma unroll
-          for (int i = 0; i < KC; ++i) {
-            const uint4 x = kr[ns][i][0], y = kr[ns][i][1];
-            mma_t<T>(d0, x.x, y.x, x.y, y.y, qf[nt][i][0], qf[nt][i][1]);
-            mma_t<T>(d1, x.z, y.z, x.w, y.w, qf[nt][i][2], qf[nt][i][3]);
+          for (int ns = 0; ns < NS; ++ns) {
+            const uint4 y = kr[ns][i][0], z = kr[ns][i][1];
+            mma_t<T>(sc[ns][nt], y.x, z.x, y.y, z.y, qf.x, qf.y);
+            mma_t<T>(NS * NT <= 2 ? sd[ns][nt] : sc[ns][nt], y.z, z.z, y.w, z.w, qf.z, qf.w);
           }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[ns][nt][e] = (d0[e] + d1[e]) * a.scale_log2;
         }
+      const int s_cur = s;
       int cur[NS];
       bool whole = s + kStep - 1 <= first_p && s >= all_lo;
 #pragma unroll
       for (int ns = 0; ns < NS; ++ns) {
         cur[ns] = pid[ns];
         whole = whole && static_cast<uint32_t>(cur[ns]) < static_cast<uint32_t>(a.num_pages);
-        pid[ns] = nxt[ns];
       }
-      const int s_next = s + kWarps * kStep;
-      load_k(s_next, pid);
-      pages_of(s_next + kWarps * kStep, nxt);
+      advance();
+      load_k(pid);
+      pages_of(row_table, s + kStride, s_end, nxt);
+#pragma unroll
+      for (int ns = 0; ns < NS; ++ns)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            sc[ns][nt][e] = (NS * NT <= 2 ? sc[ns][nt][e] + sd[ns][nt][e] : sc[ns][nt][e]) * a.scale_log2;
       if (!whole) {
 #pragma unroll
         for (int ns = 0; ns < NS; ++ns) {
-          const int st = s + 16 * ns;
+          const int st = s_cur + 16 * ns;
           const bool ok = static_cast<uint32_t>(cur[ns]) < static_cast<uint32_t>(a.num_pages);
-          if (!ok && st < s_end && lane == 0) atomicOr(&g_attn_status, RNB_STATUS_BAD_INDEX);
+          if (!ok && st < seg_end && lane == 0) atomicOr(&g_attn_status, RNB_STATUS_BAD_INDEX);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int t = st + g + 8 * (e >> 1);
-              if (!ok || t >= s_end || t > seen_hi[nt][e & 1] || t < seen_lo[nt][e & 1]) sc[ns][nt][e] = -INFINITY;
+              if (!ok || t >= seg_end || t > seen_hi[nt][e & 1] || t < seen_lo[nt][e & 1]) sc[ns][nt][e] = -INFINITY;
             }
           // values that no row of the tile sees: their bits must not count
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int t = st + 2 * c + (e & 1) + 8 * (e >> 1);
-            if (t >= s_end || t < any_lo) {
+            if (t >= seg_end || t < any_lo) {
 #pragma unroll
               for (int i = 0; i < VC; ++i) vr[ns][i][e] = make_uint4(0, 0, 0, 0);
             }
@@ -394,8 +480,17 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
           }
         }
       }
-      load_v(s_next, pid);
+      load_v(pid);
     }
+    if (!entered) {  // this warp had no step here
+      s = seg_end;
+      advance();
+      load_k(pid);
+      load_v(pid);
+      pages_of(row_table, s + kStride, s_end, nxt);
+    }
+    cp_async_wait_all();
+    if (dealer) deal(sm.seg[(x + 2) % 3]);
 
     // ---- join the four warps
 #pragma unroll
@@ -416,12 +511,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
                 make_float2(o[nt][i][j][e], o[nt][i][j][e + 2]);
       }
     __syncthreads();
-    const bool begins = blk == 0, ends = blk + n == rq.nblk;
+    const bool begins = sg.blk == 0, ends = sg.blk + sg.n == sg.nblk;
     const int part = 2 * blockIdx.x + (begins ? 1 : 0);
     float* part_ml = reinterpret_cast<float*>(a.ws + a.ml_off) + static_cast<int64_t>(part) * R * 2;
     float* part_o = reinterpret_cast<float*>(a.ws + a.o_off) + static_cast<int64_t>(part) * R * D;
-    for (int x = tid; x < R * (D / 4); x += kThreads) {
-      const int r = x / (D / 4), d = (x - r * (D / 4)) * 4;
+    for (int y = tid; y < R * (D / 4); y += kThreads) {
+      const int r = y / (D / 4), d = (y - r * (D / 4)) * 4;
+      if (row0 + r >= work) break;  // (rows ascend)
       float mx = sm.m[0][r];
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, sm.m[w][r]);
@@ -437,23 +533,22 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
         ls = fmaf(sm.l[w][r], wf, ls);
       }
       if (begins && ends) {
-        const int row = tile * R + r;
-        if (row < work) attn_write_row<T, D>(a, rq.q0 + row / a.group, h * a.group + row % a.group, d, acc, mx, ls);
+        const int row = row0 + r;
+        attn_write_row<T, D>(a, sg.q0 + row / a.group, sg.h * a.group + row % a.group, d, acc, mx, ls);
       } else {
         *reinterpret_cast<float4*>(part_o + r * D + d) = acc;
         if (d == 0) part_ml[2 * r] = mx, part_ml[2 * r + 1] = ls;
       }
     }
     if (begins && !ends && tid == 0) {
-      const int64_t tile_end = u + (rq.nblk - blk);  // first unit behind the tile
+      // (a tile that is begun and not ended is the CTA's last: its units end
+      // nblk - n behind the CTA's own)
       Begun bg;
-      bg.last = static_cast<int>((tile_end - 1) / share);
-      bg.q0 = rq.q0, bg.work = work, bg.h = h, bg.tile = tile;
+      bg.last = static_cast<int>((u1 + (sg.nblk - sg.n) - 1) / share);
+      bg.q0 = sg.q0, bg.work = work, bg.h = sg.h, bg.tile = sg.tile;
       begun[blockIdx.x] = bg;
     }
     __syncthreads();  // the join's shared memory is free again
-    rem += n;
-    u += n;
   }
   griddep_launch_dependents();
 }
@@ -510,17 +605,19 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
 }
 
 struct Plan {
-  int R, grid;
+  int R, grid, rows;  // rows a tile, CTAs, rows that a tile can have in use
   size_t ml_off, o_off, bytes;
 };
 
-Plan plan_of(const rnb_attn_desc* d, const rnb_kv_cache* c, int sms) {
+Plan plan_of(const rnb_attn_desc* d, const rnb_kv_cache* c, int sms, bool cu_given) {
   Plan p;
   const int64_t group = d->n_q_heads / c->n_kv_heads;
-  const int64_t most = d->max_q > 0 ? d->max_q : d->T > d->B ? d->T : 1;  // rows of one request
+  // rows of one request, as far as they are known
+  const int64_t most = !cu_given ? 1 : d->max_q > 0 ? d->max_q : d->T > d->B ? d->T : 1;
   // 8 rows where all fit (half the registers and products of 16); heads of 256
   // always, since 16 of them do not fit the registers
   p.R = c->head_dim == 256 || most * group <= 8 ? 8 : 16;
+  p.rows = static_cast<int>(!cu_given && group < p.R ? group : p.R);
   p.grid = 2 * sms;
   p.ml_off = (sizeof(Begun) * p.grid + 255) & ~size_t(255);
   p.o_off = (p.ml_off + 2u * p.grid * p.R * 2 * sizeof(float) + 255) & ~size_t(255);
@@ -529,12 +626,12 @@ Plan plan_of(const rnb_attn_desc* d, const rnb_kv_cache* c, int sms) {
 }
 
 template <typename T, int D, int NT>
-int run_few(AttnArgs a, int grid, cudaStream_t st) {
+int run_few(const AttnArgs& a, int grid, int rows, cudaStream_t st) {
   k_attn_few<T, D, NT><<<grid, kThreads, 0, st>>>(a);
   int rc = launch_status("rnb_paged_attention");
   if (rc) return rc;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid, 8 * NT);
+  cfg.gridDim = dim3(grid, rows);
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute at{};
@@ -548,10 +645,10 @@ int run_few(AttnArgs a, int grid, cudaStream_t st) {
 }
 
 template <typename T>
-int run_few_typed(const AttnArgs& a, int D, int R, int grid, cudaStream_t st) {
-  if (D == 256) return run_few<T, 256, 1>(a, grid, st);
-  if (D == 128) return R == 8 ? run_few<T, 128, 1>(a, grid, st) : run_few<T, 128, 2>(a, grid, st);
-  return R == 8 ? run_few<T, 64, 1>(a, grid, st) : run_few<T, 64, 2>(a, grid, st);
+int run_few_typed(const AttnArgs& a, int D, const Plan& p, cudaStream_t st) {
+  if (D == 256) return run_few<T, 256, 1>(a, p.grid, p.rows, st);
+  if (D == 128) return p.R == 8 ? run_few<T, 128, 1>(a, p.grid, p.rows, st) : run_few<T, 128, 2>(a, p.grid, p.rows, st);
+  return p.R == 8 ? run_few<T, 64, 1>(a, p.grid, p.rows, st) : run_few<T, 64, 2>(a, p.grid, p.rows, st);
 }
 
 int check_attn(const rnb_attn_desc* d, const rnb_kv_cache* c) {
@@ -588,7 +685,7 @@ int rnb_paged_attention_workspace_size(const rnb_attn_desc* d, const rnb_kv_cach
   int rc = check_attn(d, cache);
   if (rc) return rc;
   const int sms = dev_info().sms;
-  *bytes = plan_of(d, cache, sms > 0 ? sms : 148).bytes;
+  *bytes = plan_of(d, cache, sms > 0 ? sms : 148, true).bytes;
   return RNB_OK;
 }
 
@@ -606,7 +703,7 @@ int rnb_paged_attention(const rnb_attn_desc* d, const rnb_kv_cache* cache, const
   if (!aligned16(q) || !aligned16(gate) || !aligned16(out) || !aligned16(ws))
     return fail(RNB_ERR_ALIGN, "rnb_paged_attention: q, gate, out and the workspace must be 16-byte aligned");
   if ((rc = check_device())) return rc;
-  const Plan p = plan_of(d, cache, dev_info().sms);
+  const Plan p = plan_of(d, cache, dev_info().sms, cu_q != nullptr);
   if (!ws || ws_bytes < p.bytes)
     return fail(RNB_ERR_WORKSPACE, "rnb_paged_attention: the workspace needs " + std::to_string(p.bytes) + " bytes");
 
@@ -637,8 +734,8 @@ int rnb_paged_attention(const rnb_attn_desc* d, const rnb_kv_cache* cache, const
       if ((rc = run_prompt(a, cache, maps, st))) return rc;
     }
   }
-  return cache->dtype == RNB_DTYPE_BF16 ? run_few_typed<__nv_bfloat16>(a, cache->head_dim, p.R, p.grid, st)
-                                        : run_few_typed<__half>(a, cache->head_dim, p.R, p.grid, st);
+  return cache->dtype == RNB_DTYPE_BF16 ? run_few_typed<__nv_bfloat16>(a, cache->head_dim, p, st)
+                                        : run_few_typed<__half>(a, cache->head_dim, p, st);
 }
 
 }  // extern "C"
