@@ -28,53 +28,34 @@ import torch
 
 from . import _lib
 
-_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
-_i32 = torch.int32
+_calls = None  # the extension module (csrc/rnb_torch.cpp), bound to the loaded library
+
+
+def _native():
+    """The calls on torch tensors, bound once to the C functions of ``librnb_moe.so``."""
+    global _calls
+    if _calls is None:
+        lib = _lib.load()
+        try:
+            from . import _torch_calls
+        except ImportError as e:
+            raise RuntimeError("runnel_b200/_torch_calls.so is missing or does not load: build it first (python -c "
+                               "'import __graft_entry__ as g; g.build()' or make -C runnel_b200/csrc)") from e
+        names = ("rnb_kv_plan", "rnb_kv_release", "rnb_rope_append", "rnb_paged_attention_workspace_size",
+                 "rnb_paged_attention")
+        _torch_calls.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names})
+        _calls = _torch_calls
+    return _calls
 
 
 class KVPlan(NamedTuple):
-    """What :func:`kv_plan` says of a step (views of one buffer, int32)."""
+    """What :func:`kv_plan` says of a step (int32)."""
 
     seq_lens: torch.Tensor  # [B] cached plus new tokens
     cu_q: torch.Tensor  # [B + 1] first new-token row of each request, then their number
     positions: torch.Tensor  # [max_tokens]
     slots: torch.Tensor  # [max_tokens], -1 behind the last request's rows
     free_count: torch.Tensor  # [1] pages left on the free list
-
-
-def _ints(t: torch.Tensor, name: str, device: torch.device, shape: tuple | None = None) -> int:
-    """data_ptr of a contiguous int32 tensor on ``device``."""
-    if t.dtype is not _i32 or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor on {device}")
-    if shape is not None and t.shape != shape:
-        raise ValueError(f"{name} must have shape {list(shape)}, not {list(t.shape)}")
-    return t.data_ptr()
-
-
-def _cuda(t: torch.Tensor, name: str) -> torch.device:
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor: the kernels have no other implementation")
-    return t.device
-
-
-_fns: dict = {}  # bound C functions by name
-_raw_stream = torch._C._cuda_getCurrentRawStream  # what current_stream(device).cuda_stream gives, 2 us sooner
-_current_device = torch._C._cuda_getDevice
-
-
-def _call(fn: str, device: torch.device, *args) -> None:
-    """One C call on the current stream of ``device``."""
-    f = _fns.get(fn)
-    if f is None:
-        f = _fns[fn] = getattr(_lib.load(), fn)
-    i = device.index
-    if i == _current_device():
-        rc = f(*args, _raw_stream(i))
-    else:
-        with torch.cuda.device(device):
-            rc = f(*args, _raw_stream(i))
-    if rc:
-        _lib.check(fn, rc)
 
 
 def kv_plan(table: torch.Tensor, ctx_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor,
@@ -95,21 +76,8 @@ def kv_plan(table: torch.Tensor, ctx_lens: torch.Tensor, new_lens: torch.Tensor,
     ``seq_lens`` = ``ctx_lens``, nothing taken) and :func:`status` has
     ``STATUS_NO_PAGES``.
     """
-    dev = _cuda(table, "table")
-    if table.dim() != 2:
-        raise ValueError("table must be [requests, columns]")
-    B, cols = table.shape
-    if max_tokens < 0:
-        raise ValueError("max_tokens must be >= 0")
-    args = (_ints(table, "table", dev), _ints(ctx_lens, "ctx_lens", dev, (B,)), _ints(new_lens, "new_lens", dev, (B,)),
-            _ints(free_pages, "free_pages", dev), free_pages.numel(), _ints(free_count, "free_count", dev, (1,)))
-    buf = torch.empty(2 * B + 2 + 2 * max_tokens, dtype=_i32, device=dev)
-    p = buf.data_ptr()
-    cu, pos = p + 4 * B, p + 8 * B + 4
-    slots = pos + 4 * max_tokens
-    _call("rnb_kv_plan", dev, B, cols, page_size, num_pages, max_tokens, *args, p, cu, pos, slots,
-          slots + 4 * max_tokens)
-    return KVPlan(*buf.split_with_sizes((B, B + 1, max_tokens, max_tokens, 1)))
+    return KVPlan(*(_calls or _native()).kv_plan(table, ctx_lens, new_lens, free_pages, free_count, page_size, num_pages,
+                                                 max_tokens))
 
 
 def kv_release(table: torch.Tensor, lens: torch.Tensor, finished: torch.Tensor, free_pages: torch.Tensor,
@@ -117,15 +85,7 @@ def kv_release(table: torch.Tensor, lens: torch.Tensor, finished: torch.Tensor, 
     """Append the pages of requests with ``finished[b] != 0`` (int32) to
     ``free_pages[:free_count]``, in place; returns (lengths with theirs 0, the
     new count).  Does nothing, with ``STATUS_NO_PAGES``, if they do not fit."""
-    dev = _cuda(table, "table")
-    if table.dim() != 2:
-        raise ValueError("table must be [requests, columns]")
-    B, cols = table.shape
-    args = (_ints(table, "table", dev), _ints(lens, "lens", dev, (B,)), _ints(finished, "finished", dev, (B,)),
-            _ints(free_pages, "free_pages", dev), free_pages.numel(), _ints(free_count, "free_count", dev, (1,)))
-    out = torch.empty(B + 1, dtype=_i32, device=dev)
-    _call("rnb_kv_release", dev, B, cols, page_size, *args, out.data_ptr(), out.data_ptr() + 4 * B)
-    return out[:B], out[B:]
+    return (_calls or _native()).kv_release(table, lens, finished, free_pages, free_count, page_size)
 
 
 def status(device=None) -> int:
@@ -137,102 +97,9 @@ def status(device=None) -> int:
     if dev.index is None:
         dev = torch.device("cuda", torch.cuda.current_device())
     out = ctypes.c_uint32()
-    _call("rnb_kv_status", dev, ctypes.byref(out))
+    with torch.cuda.device(dev):
+        _lib.call("rnb_kv_status", ctypes.byref(out), torch.cuda.current_stream(dev).cuda_stream)
     return out.value
-
-
-# ------------------------------------------------------------- tensors
-
-def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device, shape: tuple) -> torch.Tensor:
-    """``t`` itself if the kernels take its strides, else a packed copy."""
-    if t.dtype is not dtype or t.device != device:
-        raise ValueError(f"{name} must be a {dtype} tensor on {device}")
-    if t.shape != shape:
-        raise ValueError(f"{name} must have shape {list(shape)}, not {list(t.shape)}")
-    st = t.stride()
-    if st[2] == 1 and not (st[0] | st[1]) & 7 and not t.data_ptr() & 15:
-        return t
-    return torch.empty(shape, dtype=dtype, device=device).copy_(t)
-
-
-def _cache(k: torch.Tensor, v: torch.Tensor) -> _lib.RnbKvCache:
-    code = _DTYPES.get(k.dtype)
-    if code is None or v.dtype is not k.dtype:
-        raise ValueError("k_cache and v_cache must be bfloat16 or float16, both of one type")
-    if k.dim() != 4 or v.shape != k.shape or v.device != k.device:
-        raise ValueError("k_cache and v_cache must be [num_pages, n_kv_heads, page_size, head_dim] on one device")
-    N, H, P, D = k.shape
-    ks, vs = k.stride(), v.stride()
-    if ks[3] != 1 or ks[2] != D or vs[3] != 1 or vs[2] != D:
-        raise ValueError("a head's page must be contiguous in k_cache and v_cache")
-    return _lib.RnbKvCache(code, N, P, H, D, 0, k.data_ptr(), v.data_ptr(), ks[0], ks[1], vs[0], vs[1])
-
-
-def _out(out: torch.Tensor | None, like: torch.Tensor, shape: tuple, name: str = "out") -> torch.Tensor:
-    if out is None:
-        return torch.empty(shape, dtype=like.dtype, device=like.device)
-    if out.dtype is not like.dtype or out.device != like.device or out.shape != shape or not out.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {like.dtype} tensor of shape {list(shape)} on {like.device}")
-    return out
-
-
-# -------------------------------------------------------------- rotary
-
-def _rope(q, k, v, positions, inv_freq, slots, k_cache, v_cache, sections, interleaved, q_norm, k_norm, eps, out):
-    dev = _cuda(q, "q")
-    if q.dim() != 3:
-        raise ValueError("q must be [tokens, heads, head_dim]")
-    T, Hq, D = q.shape
-    dt = q.dtype
-    code = _DTYPES.get(dt)
-    if code is None:
-        raise ValueError("q must be bfloat16 or float16")
-    half = inv_freq.numel()
-    if inv_freq.dtype is not torch.float32 or inv_freq.device != dev or not inv_freq.is_contiguous():
-        raise ValueError(f"inv_freq must be a contiguous float32 tensor on {dev}")
-    sections = (half,) if sections is None else tuple(sections)
-    axes = len(sections)
-    if not 1 <= axes <= 4:
-        raise ValueError("sections must name one to four axes")
-    if positions.dtype is torch.int64:
-        positions = positions.to(_i32)
-    if positions.shape != (axes, T) and not (axes == 1 and positions.shape == (T,)):
-        if positions.shape != (T,):
-            raise ValueError(f"positions must have shape {[axes, T]} or {[T]}, not {list(positions.shape)}")
-        positions = positions.expand(axes, T).contiguous()  # text: every axis at the token's position
-    pos = _ints(positions, "positions", dev)
-    for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        if w is not None and (w.dtype is not dt or w.device != dev or w.shape != (D,) or not w.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous {dt} tensor of {D} elements on {dev}")
-    Hkv = 0
-    ks = vs = (0, 0, 1)
-    cache = kp = vp = sp = None
-    if k_cache is not None:
-        _cuda(k_cache, "k_cache")
-        if k_cache.device != dev or k_cache.dtype is not dt:
-            raise ValueError(f"k_cache and v_cache must be {dt} tensors on {dev}, like q")
-        cache = _cache(k_cache, v_cache)
-        Hkv = cache.n_kv_heads
-        if cache.head_dim != D:
-            raise ValueError("q and the cache must have one head_dim")
-        k = _rows(k, "k", dt, dev, (T, Hkv, D))
-        v = _rows(v, "v", dt, dev, (T, Hkv, D))
-        ks, vs, kp, vp = k.stride(), v.stride(), k.data_ptr(), v.data_ptr()
-        sp = _ints(slots, "slots", dev, (T,))
-    qr = _rows(q, "q", dt, dev, (T, Hq, D))
-    if out is None:
-        out = torch.empty((T, Hq, D), dtype=dt, device=dev)
-    else:
-        _out(out, q, (T, Hq, D))
-    if T == 0:
-        return out
-    qs = qr.stride()
-    d = _lib.RnbRopeDesc(code, T, Hq, Hkv, D, 2 * half, axes, 1 if interleaved else 0, sections + (0,) * (4 - axes), eps, 0,
-                         qs[0], qs[1], ks[0], ks[1], vs[0], vs[1])
-    _call("rnb_rope_append", dev, ctypes.byref(d), qr.data_ptr(), kp, vp,
-          None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), pos,
-          inv_freq.data_ptr(), sp, None if cache is None else ctypes.byref(cache), out.data_ptr())
-    return out
 
 
 def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
@@ -253,18 +120,15 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     """
     if k_cache is None or slots is None:
         raise ValueError("rope_append needs a cache and slots; rope() turns queries without them")
-    return _rope(q, k, v, positions, inv_freq, slots, k_cache, v_cache, sections, interleaved, q_norm, k_norm, eps, out)
+    return (_calls or _native()).rope(q, k, v, positions, inv_freq, slots, k_cache, v_cache, sections, interleaved, q_norm,
+                                      k_norm, eps, out)
 
 
 def rope(q: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, sections=None, interleaved: bool = False,
          norm: torch.Tensor | None = None, eps: float = 1e-6, out: torch.Tensor | None = None) -> torch.Tensor:
     """:func:`rope_append`'s norm and rotation of one tensor ``[T, heads, head_dim]``, without a cache."""
-    return _rope(q, None, None, positions, inv_freq, None, None, None, sections, interleaved, norm, None, eps, out)
-
-
-# ----------------------------------------------------------- attention
-
-_ws_bytes: dict[tuple, int] = {}  # workspace bytes by what they depend on (shapes and device)
+    return (_calls or _native()).rope(q, None, None, positions, inv_freq, None, None, None, sections, interleaved, norm,
+                                      None, eps, out)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor,
@@ -282,52 +146,5 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     behind ``cu_q[-1]`` are left as they were.  ``max_q``, a bound on the rows of one
     request, picks the kernels and is worth giving.
     """
-    dev = _cuda(q, "q")
-    if q.dim() != 3:
-        raise ValueError("q must be [tokens, heads, head_dim]")
-    T, Hq, D = q.shape
-    dt = q.dtype
-    if k_cache.device != dev or k_cache.dtype is not dt:
-        raise ValueError(f"k_cache and v_cache must be {dt} tensors on {dev}, like q")
-    cache = _cache(k_cache, v_cache)
-    if cache.head_dim != D:
-        raise ValueError("q and the cache must have one head_dim")
-    if table.dim() != 2:
-        raise ValueError("table must be [requests, columns]")
-    B, cols = table.shape
-    tp, sl = _ints(table, "table", dev), _ints(seq_lens, "seq_lens", dev, (B,))
-    cu = None
-    if cu_q is not None:
-        cu = _ints(cu_q, "cu_q", dev, (B + 1,))
-    elif T != B:
-        raise ValueError("without cu_q every request has one query row: q must have as many as table")
-    qr = _rows(q, "q", dt, dev, (T, Hq, D))
-    gp, gs = None, (0, 0, 1)
-    if gate is not None:
-        gr = _rows(gate, "gate", dt, dev, (T, Hq, D))
-        gp, gs = gr.data_ptr(), gr.stride()
-    if out is None:
-        out = torch.empty((T, Hq, D), dtype=dt, device=dev)
-    else:
-        _out(out, q, (T, Hq, D))
-    lse = torch.empty((T, Hq), dtype=torch.float32, device=dev) if return_lse else None
-    qs = qr.stride()
-    most = 0 if max_q is None else int(max_q)
-    if most < 0:
-        raise ValueError("max_q must be >= 0")
-    if cu is None:
-        most = 1
-    d = _lib.RnbAttnDesc(B, T, Hq, cols, most, window, D ** -0.5 if scale is None else scale, 0, qs[0], qs[1], gs[0], gs[1])
-    key = (dev.index, B, T, Hq, cache.n_kv_heads, D, most)
-    need = _ws_bytes.get(key)
-    if need is None:
-        n = ctypes.c_size_t()
-        with torch.cuda.device(dev):
-            _lib.call("rnb_paged_attention_workspace_size", ctypes.byref(d), ctypes.byref(cache), ctypes.byref(n))
-        if len(_ws_bytes) > 4096:
-            _ws_bytes.clear()
-        need = _ws_bytes[key] = n.value
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    _call("rnb_paged_attention", dev, ctypes.byref(d), ctypes.byref(cache), qr.data_ptr(), gp, tp, sl, cu,
-          out.data_ptr(), None if lse is None else lse.data_ptr(), ws.data_ptr(), need)
-    return (out, lse) if return_lse else out
+    return (_calls or _native()).paged_attention(q, k_cache, v_cache, table, seq_lens, cu_q, max_q, scale, window, gate, out,
+                                                 return_lse)
