@@ -19,6 +19,8 @@ Three pieces, following the reference's tooling:
   reference tests/test_checkpoint.py:149-152); the block takes them as they
   are stored (router_bits 8: codes, scales and biases), and the arrays also
   carry a bf16 dequantisation (s*q + b in fp32, rounded) for plain-torch use.
+* :func:`load_attention` builds the layer's
+  :class:`runnel_b200.attn_layers.GatedAttention` and its input norm.
 """
 from __future__ import annotations
 
@@ -356,3 +358,52 @@ def load_block(store: TensorStore, layer: int, device="cuda", E_range: tuple[int
         bt.sgu_s, bt.sgu_b = up(a["sgu_s"], True), up(a["sgu_b"], True)
         bt.sdn_s, bt.sdn_b = up(a["sdn_s"], True), up(a["sdn_b"], True)
     return bt
+
+
+def load_attention_arrays(store: TensorStore, layer: int) -> dict:
+    """numpy arrays of a full-attention layer's ``self_attn`` (weight, scales, biases of
+    each projection, the head norms) and its ``input_layernorm``, with the sizes
+    they imply: head_dim, n_heads, n_kv_heads, gated, and bits per projection."""
+    p = f"language_model.model.layers.{layer}.self_attn"
+    if f"{p}.q_proj.weight" not in store:
+        raise ValueError(f"layer {layer} has no full attention")
+    out = {"bits": {}}
+    out["q_norm"] = store.read(f"{p}.q_norm.weight")[0]
+    out["k_norm"] = store.read(f"{p}.k_norm.weight")[0]
+    D = out["q_norm"].shape[0]
+    norm = f"language_model.model.layers.{layer}.input_layernorm.weight"
+    out["norm_w"] = store.read(norm)[0]
+    H = out["norm_w"].shape[0]
+    for proj in ("q", "k", "v", "o"):
+        w, s, b = (store.read(f"{p}.{proj}_proj.{n}")[0] for n in ("weight", "scales", "biases"))
+        K = s.shape[-1] * 64
+        bits = _bits_of(w.shape[-1], K)
+        if bits == 0 or (proj != "o" and K != H) or (proj == "o" and w.shape[0] != H):
+            raise ValueError(f"{proj}_proj does not fit hidden size {H}")
+        out[proj], out["bits"][proj] = (w, s, b), bits
+    out["head_dim"] = D
+    out["n_heads"] = out["o"][1].shape[-1] * 64 // D
+    out["n_kv_heads"] = out["k"][0].shape[0] // D
+    out["gated"] = out["q"][0].shape[0] == 2 * out["n_heads"] * D
+    return out
+
+
+def load_attention(store: TensorStore, layer: int, rotary, device="cuda", eps: float = 1e-6):
+    """A full-attention layer as (:class:`runnel_b200.attn_layers.GatedAttention`, input norm weight);
+    ``rotary`` is a :class:`runnel_b200.attn_layers.RotarySpec`."""
+    import torch
+
+    from .attn_layers import GatedAttention
+    from .switch_layers import QuantizedLinear
+
+    a = load_attention_arrays(store, layer)
+
+    def up(arr):
+        if arr.dtype == np.uint32:
+            return torch.from_numpy(np.ascontiguousarray(arr).view(np.int32)).view(torch.uint32).to(device)
+        return torch.from_numpy(np.ascontiguousarray(arr).view(np.int16)).view(torch.bfloat16).to(device)
+
+    lin = {p: QuantizedLinear(*(up(t) for t in a[p]), bits=a["bits"][p]) for p in ("q", "k", "v", "o")}
+    attn = GatedAttention(lin["q"], lin["k"], lin["v"], lin["o"], up(a["q_norm"]), up(a["k_norm"]), a["head_dim"],
+                          rotary, gated=a["gated"], eps=eps)
+    return attn, up(a["norm_w"])

@@ -12,6 +12,13 @@ launch (bit-identical to ``rnb_add_rmsnorm`` + block).  With an
 :class:`runnel_b200.ep.ExpertParallel` context every block call is expert
 parallel: each rank holds its shard of every layer and all ranks end with
 the same activations.
+
+With ``attn`` (one :class:`runnel_b200.attn_layers.GatedAttention` or None a layer)
+the stack is a decoder of whole full-attention layers,
+
+    x <- x + attn_l(rms_norm'_l(x));  x <- x + block_l(rms_norm_l(x))
+
+over a :class:`runnel_b200.attn_layers.PagedKVCache`.
 """
 from __future__ import annotations
 
@@ -35,14 +42,21 @@ def add_rmsnorm(x: torch.Tensor, y: torch.Tensor | None, w: torch.Tensor, x_out:
 
 
 class LayerStack:
-    """L MoE blocks with residual adds and RMSNorms between them."""
+    """L MoE blocks with residual adds and RMSNorms between them, and before
+    each an attention layer where ``attn`` has one."""
 
     def __init__(self, layers: list[BlockTensors], norm_w: list[torch.Tensor], eps: float = RMS_EPS,
-                 ep=None, ws: Workspace | None = None):
+                 ep=None, ws: Workspace | None = None, attn: list | None = None,
+                 attn_norm_w: list | None = None):
         if len(layers) != len(norm_w) or not layers:
             raise ValueError("need one RMSNorm weight per layer")
         self.layers, self.norm_w, self.eps, self.ep = layers, norm_w, eps, ep
         self.ws = ws
+        self.attn = attn or [None] * len(layers)
+        self.attn_norm_w = attn_norm_w or [None] * len(layers)
+        if len(self.attn) != len(layers) or len(self.attn_norm_w) != len(layers) or any(
+                (a is None) != (w is None) for a, w in zip(self.attn, self.attn_norm_w)):
+            raise ValueError("need an entry of attn and attn_norm_w per layer, both given or both None")
 
     def _layer(self, bt: BlockTensors, resid, y_prev, w, resid_out, xn, y) -> None:
         """resid_out = resid + y_prev, xn = norm(resid_out) * w, y = block(xn)."""
@@ -57,17 +71,32 @@ class LayerStack:
         _lib.call("rnb_moe_block_norm_fwd", ctypes.byref(d), ep, _ptr(resid), _ptr(y_prev), _ptr(w),
                   ctypes.c_float(self.eps), _ptr(resid_out), _ptr(xn), _ptr(y), wp, wn, _stream())
 
-    def forward(self, x: torch.Tensor, out: torch.Tensor | None = None, record: list | None = None) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, out: torch.Tensor | None = None, record: list | None = None, cache=None,
+                plan=None, max_q: int | None = None, positions: torch.Tensor | None = None) -> torch.Tensor:
         """[T, H] bf16 -> [T, H] bf16.  ``record`` (a list) receives per layer
-        (norm input x, block input xn, block output y) copies, for checking."""
+        (norm input x, block input xn, block output y) copies, for checking.
+
+        With attention layers, ``cache`` and ``plan`` are the batch's cache and
+        this step's plan (``cache.plan``; T is its ``max_tokens``); attention layer i
+        of the stack uses the cache's layer i.  ``max_q``, a bound on a request's
+        rows, and ``positions`` go to the attention layers."""
         T, H = x.shape
+        if any(a is not None for a in self.attn) and (cache is None or plan is None):
+            raise ValueError("attention layers need a cache and a plan")
         if out is None:
             out = torch.empty_like(x)
         resid_bufs = (torch.empty_like(x), torch.empty_like(x))  # the residual stream, alternating
         xn = torch.empty_like(x)
         y = torch.empty_like(x)
         resid, y_prev = x, None
+        mid, n_attn = None, 0  # the residual stream between a layer's halves
         for l, bt in enumerate(self.layers):
+            if self.attn[l] is not None:
+                if mid is None:
+                    mid = torch.empty_like(x)
+                add_rmsnorm(resid, y_prev, self.attn_norm_w[l], mid, xn, self.eps)
+                resid, y_prev = mid, self.attn[l](xn, cache, n_attn, plan, max_q, positions)
+                n_attn += 1
             r_out = resid_bufs[l % 2]
             self._layer(bt, resid, y_prev, self.norm_w[l], r_out, xn, y)
             if record is not None:

@@ -1,0 +1,204 @@
+"""The full-attention layer: loaded from a checkpoint (CPU), and on the GPU each
+of its stages against 64 bits, and a stack with attention over a paged cache
+against the calls it is made of, eagerly and from a graph."""
+import numpy as np
+import pytest
+import torch
+
+from runnel_b200 import _lib, attention, attn_layers, checkpoint, ops, probes, quant, stack
+from runnel_b200.switch_layers import QuantizedLinear
+from tests import _attn_ref as ref
+
+DEV = "cuda"
+
+
+def _linear_arrays(rng, rows, K, bits):
+    w = rng.integers(0, 2 ** 32, (rows, K * bits // 32), dtype=np.uint64).astype(np.uint32)
+    s = quant.f32_to_bf16_bits(rng.uniform(0.001, 0.01, (rows, K // 64)) * (1 if bits == 4 else 1 / 16))
+    b = quant.f32_to_bf16_bits(rng.standard_normal((rows, K // 64)) * 0.01 - 7.5 * 0.0055)
+    return w, s, b
+
+
+def _write(path, rng, H, Hq, Hkv, D, bits=(4, 4, 4, 8), gated=True, layer=3):
+    p = f"language_model.model.layers.{layer}"
+    t = {f"{p}.input_layernorm.weight": (quant.f32_to_bf16_bits(1 + 0.02 * rng.standard_normal(H)), "BF16")}
+    for n in ("q_norm", "k_norm"):
+        t[f"{p}.self_attn.{n}.weight"] = (quant.f32_to_bf16_bits(1 + 0.1 * rng.standard_normal(D)), "BF16")
+    shapes = {"q": (Hq * D * (2 if gated else 1), H), "k": (Hkv * D, H), "v": (Hkv * D, H), "o": (H, Hq * D)}
+    for (proj, (rows, K)), b in zip(shapes.items(), bits):
+        for n, a in zip(("weight", "scales", "biases"), _linear_arrays(rng, rows, K, b)):
+            t[f"{p}.self_attn.{proj}_proj.{n}"] = (a, "U32" if n == "weight" else "BF16")
+    checkpoint.write_safetensors(str(path / "model.safetensors"), t)
+    return checkpoint.TensorStore(str(path))
+
+
+@pytest.mark.parametrize("gated", [True, False])
+def test_checkpoint_attention_arrays(tmp_path, gated):
+    st = _write(tmp_path, np.random.default_rng(0), 512, 8, 2, 64, gated=gated)
+    a = checkpoint.load_attention_arrays(st, 3)
+    assert (a["head_dim"], a["n_heads"], a["n_kv_heads"], a["gated"]) == (64, 8, 2, gated)
+    assert a["bits"] == {"q": 4, "k": 4, "v": 4, "o": 8}
+    assert a["q"][0].shape == (512 * (2 if gated else 1), 64) and a["o"][0].shape == (512, 128)
+    with pytest.raises(ValueError, match="no full attention"):
+        checkpoint.load_attention_arrays(st, 0)
+
+
+def test_attention_layer_on_cpu_refuses_mixed_formats(tmp_path):
+    st = _write(tmp_path, np.random.default_rng(1), 512, 8, 2, 64, bits=(4, 8, 4, 8))
+    with pytest.raises(ValueError, match="one quantization format"):
+        checkpoint.load_attention(st, 3, attn_layers.RotarySpec(rot=32), device="cpu")
+    st = _write(tmp_path, np.random.default_rng(1), 512, 8, 2, 64)
+    layer, norm = checkpoint.load_attention(st, 3, attn_layers.RotarySpec(rot=32), device="cpu")
+    assert layer.weight.shape == (2 * 512 + 256, 64) and norm.shape == (512,) and layer.inv_freq.shape == (16,)
+    bad = QuantizedLinear(layer.weight[:64], layer.scales[:64], layer.biases[:64], bits=4)
+    kv = QuantizedLinear(layer.weight[:128], layer.scales[:128], layer.biases[:128], bits=4)
+    with pytest.raises(ValueError, match="rows"):
+        attn_layers.GatedAttention(bad, kv, kv, layer.o_proj, layer.q_norm, layer.k_norm, 64, layer.rotary)
+
+
+def test_stack_checks_its_attention_layers():
+    with pytest.raises(ValueError, match="attn_norm_w"):
+        stack.LayerStack([object()], [object()], attn=[object()])
+
+
+def _cache(n_layers, Hkv, D, B, device=DEV):
+    return attn_layers.PagedKVCache(n_layers, 40, Hkv, D, B, 400, page_size=32, device=device)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gated,sections", [(True, (6, 5, 5)), (False, None)])
+def test_layer_stages_against_64_bits(tmp_path, gated, sections):
+    H, Hq, Hkv, D = 512, 8, 2, 64
+    st = _write(tmp_path, np.random.default_rng(2), H, Hq, Hkv, D, gated=gated)
+    spec = attn_layers.RotarySpec(rot=32, theta=1e6, sections=sections)
+    layer, _ = checkpoint.load_attention(st, 3, spec, device=DEV)
+    cache = _cache(1, Hkv, D, 3)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    sec = sections or (16,)
+    lens = [0, 0, 0]
+    for new in ([90, 0, 33], [1, 4, 1], [1, 1, 70]):
+        cap = sum(new) + 3
+        plan = cache.plan(torch.tensor(new, dtype=torch.int32, device=DEV), cap)
+        x = torch.randn(cap, H, generator=g, device=DEV).to(torch.bfloat16)
+        rec = {}
+        out = layer(x, cache, 0, plan, max(new), record=rec)
+        cache.commit(plan)
+        n = sum(new)
+        lens = [a + b for a, b in zip(lens, new)]
+        assert cache.lens.tolist() == lens
+        axes = plan.positions[None].expand(len(sec), -1)
+        want, tol = ref.rope(rec["q"], axes, layer.inv_freq, sec, True, layer.q_norm)
+        ref.close(rec["q_rot"][:n], want[:n], tol[:n], "q")
+        want, tol = ref.rope(rec["k"], axes, layer.inv_freq, sec, True, layer.k_norm)
+        t = 0
+        for b, m in enumerate(new):
+            got = ref.gather(cache.k[0], cache.table[b], lens[b], 32)[lens[b] - m:]
+            ref.close(got, want[t:t + m], tol[t:t + m], "k")
+            assert torch.equal(ref.gather(cache.v[0], cache.table[b], lens[b], 32)[lens[b] - m:], rec["v"][t:t + m].double())
+            t += m
+        want, _, tol, _ = ref.attention(rec["q_rot"][:n], cache.k[0], cache.v[0], cache.table, lens, new,
+                                        gate=rec["gate"][:n] if gated else None)
+        ref.close(rec["attn"][:n], want, tol, "attention")
+        # the two products: bf16 inputs, exact weights s q + b rounded once to fp16 by the product's
+        # converters (2^-11), fp32 sums over K, rounded once to bf16 (2^-8)
+        for y, xin, w in ((rec["qkv"], x, (layer.bits, layer.weight, layer.scales, layer.biases)),
+                          (out, rec["attn"].reshape(cap, -1),
+                           (layer.o_bits, layer.o_proj.weight, layer.o_proj.scales, layer.o_proj.biases))):
+            W = probes.dequant_reference(*w)
+            z, mag = xin.double() @ W.T, xin.double().abs() @ W.abs().T
+            ref.close(y, z, 1.05 * (2.0 ** -8 * z.abs() + (2.0 ** -10 + W.shape[1] * 2.0 ** -24) * mag) + 1e-30, "product")
+        assert torch.isfinite(out).all()
+    assert attention.status() == 0
+
+
+@pytest.mark.gpu
+def test_release_lets_pages_serve_again():
+    cache = attn_layers.PagedKVCache(1, 4, 1, 64, 2, 128, page_size=32)
+    new = torch.tensor([100, 28], dtype=torch.int32, device=DEV)
+    plan = cache.plan(new, 128)
+    cache.commit(plan)
+    # four pages hold 128 tokens; 100 and 28 need five: the plan was void
+    assert attention.status() == _lib.STATUS_NO_PAGES and cache.lens.tolist() == [0, 0]
+    plan = cache.plan(torch.tensor([96, 28], dtype=torch.int32, device=DEV), 128)
+    cache.commit(plan)
+    assert cache.lens.tolist() == [96, 28] and cache.free_count.item() == 0
+    first = sorted(cache.table[0, :3].tolist())
+    cache.release(torch.tensor([1, 0], dtype=torch.int32, device=DEV))
+    assert cache.lens.tolist() == [0, 28] and cache.free_count.item() == 3
+    plan = cache.plan(torch.tensor([0, 90], dtype=torch.int32, device=DEV), 128)
+    cache.commit(plan)
+    assert cache.lens.tolist() == [0, 118] and cache.free_count.item() == 0
+    assert sorted(cache.table[1, 1:4].tolist()) == first
+    assert attention.status() == 0
+
+
+def _stack(tmp_path, seed):
+    """Two MoE layers, the second with attention before it."""
+    layers, norms = stack.synthetic_layers(2, 4, seed=seed, device=DEV, H=2048, I=512, E=16)
+    st = _write(tmp_path, np.random.default_rng(seed), 2048, 16, 2, 128)
+    a, an = checkpoint.load_attention(st, 3, attn_layers.RotarySpec(rot=64, sections=(12, 10, 10)), device=DEV)
+    return stack.LayerStack(layers, norms, ws=ops.Workspace(DEV), attn=[None, a], attn_norm_w=[None, an])
+
+
+@pytest.mark.gpu
+def test_stack_with_attention_steps_and_graph(tmp_path):
+    s = _stack(tmp_path, 11)
+    steps = [[40, 0, 3], [1, 30, 1], [1, 1, 1], [1, 1, 1]]
+    cap = 64
+    g = torch.Generator(device=DEV).manual_seed(12)
+    xs = [torch.randn(cap, 2048, generator=g, device=DEV).to(torch.bfloat16) for _ in steps]
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+
+    cache = _cache(1, 2, 128, 3)
+    outs = []
+    for new, x in zip(steps, xs):
+        plan = cache.plan(ints(new), cap)
+        outs.append(s.forward(x, cache=cache, plan=plan))
+        cache.commit(plan)
+
+    # the calls it is made of
+    cache = _cache(1, 2, 128, 3)
+    a, an = s.attn[1], s.attn_norm_w[1]
+    for new, x, want in zip(steps, xs, outs):
+        plan = cache.plan(ints(new), cap)
+        r, xn = torch.empty_like(x), torch.empty_like(x)
+        stack.add_rmsnorm(x, None, s.norm_w[0], r, xn)
+        y = ops.moe_block(s.layers[0], xn)
+        stack.add_rmsnorm(r, y, an, r, xn)
+        y = a(xn, cache, 0, plan)
+        stack.add_rmsnorm(r, y, s.norm_w[1], r, xn)
+        y = ops.moe_block(s.layers[1], xn)
+        stack.add_rmsnorm(r, y, s.norm_w[1], r, xn)
+        cache.commit(plan)
+        assert torch.equal(r[:sum(new)], want[:sum(new)])
+
+    # one captured step for all of them
+    cache = _cache(1, 2, 128, 3)
+    new, x, out = ints(steps[0]), xs[0].clone(), torch.empty_like(xs[0])
+
+    def step():
+        plan = cache.plan(new, cap)
+        s.forward(x, out=out, cache=cache, plan=plan)
+        cache.commit(plan)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    cache.lens.zero_()
+    cache.free_count.fill_(40)
+    for n, xx, want in zip(steps, xs, outs):
+        new.copy_(ints(n))
+        x.copy_(xx)
+        graph.replay()
+        assert torch.equal(out[:sum(n)], want[:sum(n)])
+    assert cache.lens.tolist() == [sum(v) for v in zip(*steps)]
+    assert attention.status() == 0
+
+
+@pytest.mark.gpu
+def test_stack_refuses_attention_without_a_cache(tmp_path):
+    s = _stack(tmp_path, 13)
+    with pytest.raises(ValueError, match="cache and a plan"):
+        s.forward(torch.zeros(1, 2048, dtype=torch.bfloat16, device=DEV))
