@@ -49,7 +49,7 @@ def _native():
 
 
 class KVPlan(NamedTuple):
-    """What :func:`kv_plan` says of a step (int32)."""
+    """What :func:`kv_plan` says of a step (parts of one int32 buffer)."""
 
     seq_lens: torch.Tensor  # [B] cached plus new tokens
     cu_q: torch.Tensor  # [B + 1] first new-token row of each request, then their number

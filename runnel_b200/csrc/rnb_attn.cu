@@ -74,6 +74,12 @@ __device__ __forceinline__ void mma_t<__nv_bfloat16>(float (&d)[4], uint32_t a0,
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// ceil(a / b) without the 64-bit division wherever 32 bits do (100 cycles on
+// the way to the first load).
+__device__ __forceinline__ int64_t share_of(int64_t a, uint32_t b) {
+  return a < INT_MAX ? (static_cast<uint32_t>(a) + b - 1) / b : (a + b - 1) / b;
+}
+
 // One request's share of the work.
 struct Request {
   int q0, rows, len;      // first query row, rows, cached positions
@@ -148,7 +154,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
   bool dealer = false;
   int64_t start_rem = 0;
   int at = 0, h_at = 0, tile_at = 0, p_at = 0, c0 = 0, c1 = 0, len = 0;
-  {
+  if (!a.direct) {
     const int per = (a.B + kThreads - 1) / kThreads;
     const int lo = min(tid * per, a.B), hi = min(lo + per, a.B);
     auto units = [&](int b) {
@@ -171,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
     for (int w = 0; w < warp; ++w) base += wsum[w];
     if (tid == kThreads - 1) total = base + sum;
     __syncthreads();
-    const int64_t share = (total + gridDim.x - 1) / gridDim.x, u0 = share * blockIdx.x;
+    const int64_t share = share_of(total, gridDim.x), u0 = share * blockIdx.x;
     if (u0 >= base && u0 < base + sum) {
       dealer = true;
       start_rem = u0 - base;
@@ -182,13 +188,32 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
       }
     }
   }
-  const int64_t share = (total + gridDim.x - 1) / gridDim.x, u0 = share * blockIdx.x;
-  const int64_t u1 = min(u0 + share, total);
+  // (direct: every request has one row, so tile i is known without the lengths;
+  // this CTA takes whole tiles, gridDim.x apart)
+  const int tiles_a_head = (a.group + R - 1) / R, tiles_a_request = tiles_a_head * a.Hkv;
+  const int64_t share = a.direct ? gridDim.x : share_of(total, gridDim.x);
+  const int64_t u0 = a.direct ? blockIdx.x : share * blockIdx.x;
+  const int64_t u1 = a.direct ? static_cast<int64_t>(a.B) * tiles_a_request : min(u0 + share, total);
   if (u0 >= u1) return;
 
   int64_t u_at = u0;
   auto deal = [&](Segment& sg) {
     sg.n = 0;
+    if (a.direct) {
+      if (u_at < u1) {
+        const int i = static_cast<int>(u_at);  // (T n_q_heads fits)
+        u_at += share;
+        sg.b = i / tiles_a_request;
+        const int j = i - sg.b * tiles_a_request;
+        sg.h = j / tiles_a_head, sg.tile = j - sg.h * tiles_a_head;
+        read_request(a, sg.b, c0, c1, len);
+        if (j == 0 && (len < 0 || len > a.max_kv)) atomicOr(&g_attn_status, RNB_STATUS_BAD_INDEX);
+        const Request rq = request_of<R>(a, c0, c1, len);
+        sg.q0 = rq.q0, sg.rows = rq.rows, sg.len = rq.len, sg.blk0 = rq.blk0, sg.nblk = sg.n = rq.nblk;
+        sg.blk = 0;
+      }
+      return;
+    }
     while (u_at < u1 && at < a.B) {  // (the second: lengths that change under way must not hang it)
       const Request rq = request_of<R>(a, c0, c1, len);
       if (h_at < a.Hkv && rq.ntile > 0) {
@@ -211,12 +236,19 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
       if (sg.n > 0) return;
     }
   };
-  if (dealer) {
+  if (a.direct) {
+    dealer = tid == 0;
+    if (dealer) {
+      deal(sm.seg[0]);
+      deal(sm.seg[1]);
+    }
+  } else if (dealer) {
     const Request rq = request_of<R>(a, c0, c1, len);
     const int cost = rq.nblk + kTile;
     const int64_t tile_of = start_rem < INT_MAX ? static_cast<int>(start_rem) / cost : start_rem / cost;
     p_at = static_cast<int>(start_rem - tile_of * cost);
-    h_at = static_cast<int>(tile_of / max(rq.ntile, 1));
+    const int nt = max(rq.ntile, 1);
+    h_at = static_cast<int>(tile_of < INT_MAX ? static_cast<int>(tile_of) / nt : tile_of / nt);
     tile_at = static_cast<int>(tile_of - static_cast<int64_t>(h_at) * rq.ntile);
     deal(sm.seg[0]);
     deal(sm.seg[1]);
@@ -515,9 +547,22 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
     const int part = 2 * blockIdx.x + (begins ? 1 : 0);
     float* part_ml = reinterpret_cast<float*>(a.ws + a.ml_off) + static_cast<int64_t>(part) * R * 2;
     float* part_o = reinterpret_cast<float*>(a.ws + a.o_off) + static_cast<int64_t>(part) * R * D;
-    for (int y = tid; y < R * (D / 4); y += kThreads) {
-      const int r = y / (D / 4), d = (y - r * (D / 4)) * 4;
-      if (row0 + r >= work) break;  // (rows ascend)
+    constexpr int kPieces = R * (D / 4) / kThreads;  // of four elements, a thread
+    const bool done = begins && ends;
+    uint2 gw[kPieces];
+    if (done && a.gate) {  // all under way at once
+#pragma unroll
+      for (int y = 0; y < kPieces; ++y) {
+        const int z = y * kThreads + tid, r = z / (D / 4), row = row0 + r;
+        if (row < work)
+          gw[y] = __ldg(reinterpret_cast<const uint2*>(attn_gate<T>(a, sg.q0 + row / a.group, sg.h * a.group + row % a.group) +
+                                                       (z - r * (D / 4)) * 4));
+      }
+    }
+#pragma unroll
+    for (int y = 0; y < kPieces; ++y) {
+      const int z = y * kThreads + tid, r = z / (D / 4), d = (z - r * (D / 4)) * 4, row = row0 + r;
+      if (row >= work) break;  // (rows ascend)
       float mx = sm.m[0][r];
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, sm.m[w][r]);
@@ -532,9 +577,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
         acc.z = fmaf(v.z, wf, acc.z), acc.w = fmaf(v.w, wf, acc.w);
         ls = fmaf(sm.l[w][r], wf, ls);
       }
-      if (begins && ends) {
-        const int row = row0 + r;
-        attn_write_row<T, D>(a, sg.q0 + row / a.group, sg.h * a.group + row % a.group, d, acc, mx, ls);
+      if (done) {
+        attn_write_row<T, D>(a, sg.q0 + row / a.group, sg.h * a.group + row % a.group, d, acc, mx, ls, gw[y]);
       } else {
         *reinterpret_cast<float4*>(part_o + r * D + d) = acc;
         if (d == 0) part_ml[2 * r] = mx, part_ml[2 * r + 1] = ls;
@@ -568,6 +612,10 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
   const float* ml = reinterpret_cast<const float*>(a.ws + a.ml_off);
   const float* po = reinterpret_cast<const float*>(a.ws + a.o_off);
   auto part = [&](int i) { return static_cast<int64_t>(2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * R + r; };
+  const int col = tid % kCols, way = tid / kCols;
+  const int t = bg.q0 + row / a.group, head = bg.h * a.group + row % a.group;
+  uint2 gw = make_uint2(0, 0);
+  if (a.gate && way == 0) gw = __ldg(reinterpret_cast<const uint2*>(attn_gate<T>(a, t, head) + 4 * col));
   float mx = -INFINITY;
   for (int i = tid; i < n; i += 256) mx = fmaxf(mx, ml[2 * part(i)]);
   mx = warp_max(mx);
@@ -576,9 +624,9 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
 #pragma unroll
   for (int w = 0; w < 8; ++w) mx = fmaxf(mx, red[w]);
   const float use = mx == -INFINITY ? 0.f : mx;
-  const int col = tid % kCols, way = tid / kCols;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float ls = 0.f;
+#pragma unroll 4
   for (int i = way; i < n; i += kWays) {
     const int64_t p = part(i);
     const float f = ex2(ml[2 * p] - use);
@@ -600,7 +648,7 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
     ls = lred[0];
 #pragma unroll
     for (int w = 1; w < kWays; ++w) ls += lred[w];
-    attn_write_row<T, D>(a, bg.q0 + row / a.group, bg.h * a.group + row % a.group, 4 * col, acc, mx, ls);
+    attn_write_row<T, D>(a, t, head, 4 * col, acc, mx, ls, gw);
   }
 }
 
@@ -627,6 +675,11 @@ Plan plan_of(const rnb_attn_desc* d, const rnb_kv_cache* c, int sms, bool cu_giv
 
 template <typename T, int D, int NT>
 int run_few(const AttnArgs& a, int grid, int rows, cudaStream_t st) {
+  if (a.direct) {
+    const int64_t tiles = static_cast<int64_t>(a.B) * a.Hkv * ((a.group + 8 * NT - 1) / (8 * NT));
+    k_attn_few<T, D, NT><<<static_cast<unsigned>(tiles < grid ? tiles : grid), kThreads, 0, st>>>(a);
+    return launch_status("rnb_paged_attention");
+  }
   k_attn_few<T, D, NT><<<grid, kThreads, 0, st>>>(a);
   int rc = launch_status("rnb_paged_attention");
   if (rc) return rc;
@@ -726,6 +779,12 @@ int rnb_paged_attention(const rnb_attn_desc* d, const rnb_kv_cache* cache, const
   a.few_rows = INT32_MAX;
   a.scale_log2 = d->scale * 1.4426950408889634f;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // One row a request and short tables: whole tiles, without the sums over the
+  // requests and without the join (one request at head_dim 128: 256 positions 8.8 ->
+  // 6.6 us, 64 at head_dim 256 10.2 -> 6.4).  A CTA walks a tile at 1.3 us a 64 KB of keys
+  // and values, so longer ones are split; at this border (224 positions of 256, 448 of
+  // 128) both take the same.
+  a.direct = !cu_q && static_cast<int64_t>(a.max_kv) * cache->head_dim <= 224 * 256;
   const int64_t most = cu_q ? (d->max_q > 0 ? d->max_q : d->T) : 1;
   if (cu_q && most * a.group >= kManyRows) {
     PromptMaps maps;

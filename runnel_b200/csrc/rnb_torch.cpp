@@ -85,6 +85,16 @@ Tensor empty(at::IntArrayRef shape, at::ScalarType dt, at::Device dev) {
   return at::detail::empty_cuda(shape, dt, dev, std::nullopt);
 }
 
+// n elements of a one-dimensional buffer, sharing its storage (as narrow() gives,
+// without its dispatch).
+Tensor part(const Tensor& buf, int64_t off, int64_t n) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(buf.storage()), buf.key_set(),
+                                                      buf.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(buf.storage_offset() + off);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return t;
+}
+
 // A [tokens, heads, head_dim] operand: itself if the kernels take its strides,
 // else a packed copy.
 struct Rows {
@@ -155,8 +165,13 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> kv_plan(const Tensor& table, 
   const int32_t* fp = ints(free_pages, "free_pages", dev);
   const int32_t* fc = ints(free_count, "free_count", dev, {1});
   const c10::cuda::CUDAGuard guard(dev);
-  Tensor seq = empty({B}, at::kInt, dev), cu = empty({B + 1}, at::kInt, dev), pos = empty({max_tokens}, at::kInt, dev),
-         slots = empty({max_tokens}, at::kInt, dev), left = empty({1}, at::kInt, dev);
+  // one allocation; each output starts 16 bytes aligned
+  const int64_t n[5] = {B, B + 1, max_tokens, max_tokens, 1};
+  int64_t off[5], all = 0;
+  for (int i = 0; i < 5; ++i) off[i] = all, all += (n[i] + 3) & ~int64_t(3);
+  const Tensor buf = empty({all}, at::kInt, dev);
+  Tensor seq = part(buf, off[0], n[0]), cu = part(buf, off[1], n[1]), pos = part(buf, off[2], n[2]),
+         slots = part(buf, off[3], n[3]), left = part(buf, off[4], n[4]);
   auto p = [](Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); };
   check("rnb_kv_plan", fns.kv_plan(c_int(B, "requests"), c_int(cols, "columns"), c_int(page_size, "page_size"),
                                    c_int(num_pages, "num_pages"), c_int(max_tokens, "max_tokens"), tp, cp, np, fp,

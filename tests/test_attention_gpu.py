@@ -315,6 +315,28 @@ def test_one_token_each(dtype, Hq, Hkv, D):
     assert attention.status() == 0
 
 
+@pytest.mark.parametrize("Hq,Hkv,D", HEADS)
+@pytest.mark.parametrize("B", [1, 7, 700])
+def test_one_token_each_over_short_tables(Hq, Hkv, D, B):
+    """Tables short enough that whole tiles are dealt by number, up to more tiles than CTAs."""
+    g = _gen(B + D)
+    r = random.Random(B)
+    lens = [r.choice([0, 1, 16, 17, 63, 64, 100, 127]) for _ in range(B)]
+    lens[0] = 127
+    kc, vc, table = _cache_of(g, BF16, lens, Hkv, D, 16)
+    q = _rand(g, BF16, B, Hq, D, scale=1.5)
+    gate = _rand(g, BF16, B, Hq, D)
+    few = min(B, 40)  # the rows that are checked
+    want, wlse, tol, ltol = ref.attention(q[-few:], kc, vc, table[-few:], lens[-few:], [1] * few, gate=gate[-few:], window=70)
+    out, lse = attention.paged_attention(q, kc, vc, table, _i(lens), gate=gate, window=70, return_lse=True)
+    ref.close(out[-few:], want, tol, "out")
+    ref.close(lse[-few:], wlse, ltol, "lse")
+    long = torch.cat([table, torch.full((B, 64), 2 ** 30, dtype=torch.int32, device=DEV)], 1)
+    alike, _ = attention.paged_attention(q, kc, vc, long, _i(lens), gate=gate, window=70, return_lse=True)
+    ref.close(alike[-few:], want, tol, "the same over a long table")
+    assert attention.status() == 0
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("Hq,Hkv,D", HEADS)
 @pytest.mark.parametrize("max_q", [None, 5])
