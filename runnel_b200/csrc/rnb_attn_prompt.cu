@@ -209,7 +209,8 @@ struct Bars {
   uint64_t q_full;              // Q in shared memory
   uint64_t q_done;              // every product with Q done
   uint64_t g_full;              // the gates where Q was
-  uint64_t s_full[4], p_full[4];  // slots: S written, P written (S read)
+  uint64_t s_full[2];           // slots: S written
+  uint64_t p_full[2][2];        // slots: each half of P written (S read)
   uint64_t o_done[2];           // row tiles: a P V product done
   uint64_t o_last[2];           // row tiles: the last one done
   uint64_t drained;             // every product of the CTA done
@@ -300,7 +301,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     mbar_init(&bars.drained, 1);
     for (int i = 0; i < C::NS; ++i) {
       mbar_init(&bars.s_full[i], 1);
-      mbar_init(&bars.p_full[i], 4);
+      mbar_init(&bars.p_full[i][0], 4);
+      mbar_init(&bars.p_full[i][1], 4);
     }
     for (int i = 0; i < C::NQ; ++i) {
       mbar_init(&bars.o_done[i], 1);
@@ -438,16 +440,18 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
           fence_proxy_async_smem();
           __syncwarp();
         }
-        if (part == 0) {
-          alive = wait_on(&bars.p_full[k % C::NS], (k / C::NS) & 1);
-          if (!alive) return;
-        }
-        tc_fence_after();
         const uint64_t vd = umma_desc_mn(rbase + st * C::kUnit, C::VR * 128);
 #pragma unroll
-        for (int s = 0; s < C::VR / 16; ++s)
-          umma_ts(leader, tmem + C::kTmemO + q * D, tmem + (k % C::NS) * C::BN + (part * C::VR + s * 16) / 2,
-                  vd + (s * 16 * 128 >> 4), id_o, i != 0 || part != 0 || s != 0);
+        for (int s = 0; s < C::VR / 16; ++s) {
+          const int t = part * C::VR + s * 16;
+          if (t % 64 == 0) {  // the first half's products run while the second half of P is computed
+            alive = wait_on(&bars.p_full[k % C::NS][t / 64], (k / C::NS) & 1);
+            if (!alive) return;
+            tc_fence_after();
+          }
+          umma_ts(leader, tmem + C::kTmemO + q * D, tmem + (k % C::NS) * C::BN + t / 2, vd + (s * 16 * 128 >> 4), id_o,
+                  i != 0 || t != 0);
+        }
         if (leader) {
           if (C::NQ == 1 || q == 1) umma_commit(smem_u32(&bars.empty[st]));
           if (part == C::UPT - 1) umma_commit(smem_u32(i + 1 < nblk ? &bars.o_done[q] : &bars.o_last[q]));
@@ -507,7 +511,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
       for (int c = 0; c < NC; ++c) tmem_ld32(t_s + 32 * c, v[c]);
       tmem_wait_ld();
       const int t0 = (blk0 + i) * C::BN;
-      if (bad || t0 + C::BN - 1 > wg_first || t0 < all_lo) {
+      if (__builtin_expect(bad || t0 + C::BN - 1 > wg_first || t0 < all_lo, 0)) {
         const int hi = pos - t0, lo = see_lo - t0;
 #pragma unroll
         for (int c = 0; c < NC; ++c)
@@ -577,12 +581,14 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
           p[e] = Pair<T>::pack(y.x, y.y);
         }
         tmem_st16(t_s + 16 * c, p);
+        if (c & 1) {  // a half of P
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars.p_full[slot][c >> 1]);
+        }
       }
       l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.p_full[slot]);
     }
     // ---- O / l
     // (o_done would not do: the last two products may both be under way, and a
