@@ -683,6 +683,7 @@ int run_few(const AttnArgs& a, int grid, int rows, cudaStream_t st) {
   k_attn_few<T, D, NT><<<grid, kThreads, 0, st>>>(a);
   int rc = launch_status("rnb_paged_attention");
   if (rc) return rc;
+  // (its launch overlaps the first kernel's end; it waits for that itself)
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(grid, rows);
   cfg.blockDim = dim3(256);
@@ -789,8 +790,10 @@ int rnb_paged_attention(const rnb_attn_desc* d, const rnb_kv_cache* cache, const
   if (cu_q && most * a.group >= kManyRows) {
     PromptMaps maps;
     if (prepare_prompt(a, cache, &maps)) {
-      a.few_rows = kManyRows;
+      // (a single request is wholly the many-row kernel's, however few its rows are)
+      a.few_rows = d->B == 1 ? 1 : kManyRows;
       if ((rc = run_prompt(a, cache, maps, st))) return rc;
+      if (d->B == 1) return RNB_OK;
     }
   }
   return cache->dtype == RNB_DTYPE_BF16 ? run_few_typed<__nv_bfloat16>(a, cache->head_dim, p, st)

@@ -361,6 +361,25 @@ def test_prompts(Hq, Hkv, D, dtype):
     _check_attention(q, kc, vc, table, lens, rows, gate=gate)
 
 
+@pytest.mark.parametrize("n,r", [(1, 1), (70, 1), (300, 3), (40, 64), (257, 200), (0, 5), (130, 0)])
+@pytest.mark.parametrize("Hq,Hkv,D", [(16, 2, 256), (7, 1, 128), (64, 1, 64), (200, 1, 64)])
+def test_a_single_request_of_any_rows(n, r, Hq, Hkv, D):
+    """One request, its rows known to the device alone; padding behind them stays."""
+    g = _gen(n + r)
+    kc, vc, table = _cache_of(g, BF16, [n], Hkv, D, 16)
+    q = _rand(g, BF16, r + 70, Hq, D)
+    gate = _rand(g, BF16, r + 70, Hq, D)
+    for window in (0, 33):
+        out = torch.full_like(q, 9.0)
+        got, lse = attention.paged_attention(q, kc, vc, table, _i([n]), cu_q=_i([0, r]), gate=gate, window=window,
+                                             out=out, return_lse=True)
+        want, wlse, tol, ltol = ref.attention(q[:r], kc, vc, table, [n], [r], gate=gate[:r], window=window)
+        ref.close(out[:r], want, tol, "out")
+        ref.close(lse[:r], wlse, ltol, "lse")
+        assert got is out and (out[r:] == 9).all()
+    assert attention.status() == 0
+
+
 @pytest.mark.parametrize("window", [1, 7, 16, 64, 100, 1000])
 @pytest.mark.parametrize("rows", [[1, 1, 1, 1], [3, 1, 150, 70]])
 def test_windows(window, rows):
