@@ -138,6 +138,7 @@ struct Steps {
 
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
+  after_previous();
   constexpr int R = 8 * NT, NS = Steps<D, NT>::NS, KC = D / 32, VC = D / 64;
   constexpr int kStep = 16 * NS, kStride = kWarps * kStep;
   constexpr int kTile = 512 / D;  // what starting and joining a tile costs, in units (without it
@@ -594,7 +595,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
     }
     __syncthreads();  // the join's shared memory is free again
   }
-  griddep_launch_dependents();
 }
 
 // Block (i, r): row r of the tile that CTA i of the kernel above began, from the
@@ -604,7 +604,7 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
   constexpr int kCols = D / 4, kWays = 256 / kCols;
   __shared__ float4 acc_s[kWays][kCols];
   __shared__ float red[8], lred[kWays];
-  griddep_wait();
+  after_previous();
   const Begun bg = reinterpret_cast<const Begun*>(a.ws)[blockIdx.x];
   const int r = blockIdx.y, row = bg.tile * R + r;
   if (bg.last < 0 || row >= bg.work) return;
@@ -675,27 +675,11 @@ Plan plan_of(const rnb_attn_desc* d, const rnb_kv_cache* c, int sms, bool cu_giv
 
 template <typename T, int D, int NT>
 int run_few(const AttnArgs& a, int grid, int rows, cudaStream_t st) {
-  if (a.direct) {
-    const int64_t tiles = static_cast<int64_t>(a.B) * a.Hkv * ((a.group + 8 * NT - 1) / (8 * NT));
-    k_attn_few<T, D, NT><<<static_cast<unsigned>(tiles < grid ? tiles : grid), kThreads, 0, st>>>(a);
-    return launch_status("rnb_paged_attention");
-  }
-  k_attn_few<T, D, NT><<<grid, kThreads, 0, st>>>(a);
-  int rc = launch_status("rnb_paged_attention");
-  if (rc) return rc;
-  // (its launch overlaps the first kernel's end; it waits for that itself)
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid, rows);
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, k_attn_join<T, D, 8 * NT>, a);
-  if (e != cudaSuccess) return fail(RNB_ERR_CUDA, std::string("rnb_paged_attention join: ") + cudaGetErrorString(e));
-  return RNB_OK;
+  const int64_t tiles = static_cast<int64_t>(a.B) * a.Hkv * ((a.group + 8 * NT - 1) / (8 * NT));
+  const unsigned ctas = static_cast<unsigned>(a.direct && tiles < grid ? tiles : grid);
+  const int rc = launch("rnb_paged_attention", k_attn_few<T, D, NT>, ctas, kThreads, 0, st, a);
+  if (rc || a.direct) return rc;
+  return launch("rnb_paged_attention join", k_attn_join<T, D, 8 * NT>, dim3(grid, rows), 256, 0, st, a);
 }
 
 template <typename T>

@@ -219,6 +219,7 @@ struct Bars {
 template <typename T, int D>
 __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     k_attn_prompt(const AttnArgs a, const __grid_constant__ PromptMaps maps) {
+  after_previous();
   using C = Cfg<D>;
   extern __shared__ char raw[];
   __shared__ Bars bars;
@@ -670,8 +671,8 @@ int launch_prompt(const AttnArgs& a, const PromptMaps& maps, cudaStream_t st) {
   const int64_t per = static_cast<int64_t>(maps.tokens) * C::NQ;
   const int64_t tiles = (a.T + per - 1) / per + (a.B < a.T ? a.B : a.T);
   if (tiles * a.Hkv > INT32_MAX) return fail(RNB_ERR_INVALID, "rnb_paged_attention: too many rows");
-  k_attn_prompt<T, D><<<static_cast<unsigned>(tiles * a.Hkv), C::kThreads, C::kSmem, st>>>(a, maps);
-  return launch_status("rnb_paged_attention");
+  return launch("rnb_paged_attention", k_attn_prompt<T, D>, static_cast<unsigned>(tiles * a.Hkv), C::kThreads, C::kSmem, st,
+                a, maps);
 }
 
 bool encode_cache(CUtensorMap* m, const rnb_kv_cache* c, const void* base, int64_t page_stride, int64_t head_stride,

@@ -35,7 +35,7 @@ __device__ uint32_t g_kv_status;
 // block calls it.
 __device__ void block_sums(int32_t* a, int32_t* b, int n, int64_t (*wsum)[2], int64_t* tot) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int per = (n + kPlanThreads - 1) / kPlanThreads;
+  const int per = ((n + kPlanThreads - 1) / kPlanThreads) | 1;  // odd: no bank conflicts between the threads' parts
   const int lo = min(tid * per, n), hi = min(lo + per, n);
   int64_t sa = 0, sb = 0;
   for (int i = lo; i < hi; ++i) {
@@ -98,6 +98,7 @@ struct PlanArgs {
 };
 
 __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(const PlanArgs a) {
+  after_previous();
   extern __shared__ int32_t sh[];
   int32_t* cu = sh;           // [B] first token row of each request
   int32_t* base = sh + a.B;   // [B] first new page of each request
@@ -131,14 +132,14 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(const PlanArgs a) {
   }
   for (int n = at; n < pages; n += stride) {
     const int b = find_request(base, a.B, n);
-    const int held = (a.ctx[b] + P - 1) >> a.log2p;
+    const int held = static_cast<int>((static_cast<int64_t>(a.ctx[b]) + P - 1) >> a.log2p);
     a.table[static_cast<int64_t>(b) * a.W + held + (n - base[b])] = a.free_pages[fc - 1 - n];
   }
   for (int t = at; t < a.max_tokens; t += stride) {
     int pos = 0, slot = -1;
     if (t < tokens) {
       const int b = find_request(cu, a.B, t);
-      const int c = a.ctx[b], held = (c + P - 1) >> a.log2p;
+      const int c = a.ctx[b], held = static_cast<int>((static_cast<int64_t>(c) + P - 1) >> a.log2p);
       pos = c + (t - cu[b]);
       const int j = pos >> a.log2p;
       const int page = j < held ? a.table[static_cast<int64_t>(b) * a.W + j] : a.free_pages[fc - 1 - (base[b] + j - held)];
@@ -163,6 +164,7 @@ struct ReleaseArgs {
 // One CTA (requests finish one at a time): the pages of all finished requests
 // as one flat range, each found by binary search.
 __global__ void __launch_bounds__(kPlanThreads) k_kv_release(const ReleaseArgs a) {
+  after_previous();
   extern __shared__ int32_t sh[];
   int32_t* base = sh;        // [B]
   int32_t* none = sh + a.B;  // [B] the second of block_sums' arrays
@@ -255,8 +257,7 @@ int rnb_kv_plan(int B, int table_cols, int page_size, int num_pages, int max_tok
   grid = grid < 1 ? 1 : grid > sms ? sms : grid;
   const PlanArgs a{B, table_cols, log2_of(page_size), num_pages, max_tokens, free_capacity, table, ctx_lens, new_lens,
                    free_pages, free_count, seq_lens, cu_q, positions, slots, free_count_out};
-  k_kv_plan<<<grid, kPlanThreads, smem, static_cast<cudaStream_t>(stream)>>>(a);
-  return launch_status("rnb_kv_plan");
+  return launch("rnb_kv_plan", k_kv_plan, grid, kPlanThreads, smem, static_cast<cudaStream_t>(stream), a);
 }
 
 int rnb_kv_release(int B, int table_cols, int page_size, const int32_t* table, const int32_t* lens,
@@ -276,8 +277,7 @@ int rnb_kv_release(int B, int table_cols, int page_size, const int32_t* table, c
   if ((rc = allow_smem(k_kv_release, smem))) return rc;
   const ReleaseArgs a{B, table_cols, log2_of(page_size), free_capacity, table, lens, finished, free_pages, free_count,
                       lens_out, free_count_out};
-  k_kv_release<<<1, kPlanThreads, smem, static_cast<cudaStream_t>(stream)>>>(a);
-  return launch_status("rnb_kv_release");
+  return launch("rnb_kv_release", k_kv_release, 1, kPlanThreads, smem, static_cast<cudaStream_t>(stream), a);
 }
 
 int rnb_kv_status(uint32_t* status, void* stream) {

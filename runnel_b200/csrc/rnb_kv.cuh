@@ -39,10 +39,33 @@ inline int check_cache(const rnb_kv_cache* c, const char* fn) {
   return RNB_OK;
 }
 
-inline int launch_status(const char* what) {
-  const cudaError_t e = cudaGetLastError();
+// A launch whose grid may come up while the kernel before it in the stream ends
+// (programmatic dependent launch; 1 us less between two small kernels).  Every
+// kernel launched so waits for that one (griddep_wait) before anything else, its
+// early returns included, so that "this grid is done" still means that all before
+// it are.
+template <typename... P, typename... A>
+inline int launch(const char* what, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                  const A&... args) {
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
   if (e != cudaSuccess) return fail(RNB_ERR_CUDA, std::string(what) + " launch: " + cudaGetErrorString(e));
   return RNB_OK;
+}
+
+// First thing in such a kernel.
+__device__ __forceinline__ void after_previous() {
+  griddep_wait();
+  griddep_launch_dependents();
 }
 
 // Reads and clears one unit's device status word (synchronises the stream).

@@ -145,6 +145,7 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeCtas) k_rope_append(const R
   constexpr int kLanes = D / 8;                   // lanes holding one head's row
   constexpr int kGroups = kRopeThreads / kLanes;  // rows in flight in the CTA
   __shared__ __align__(16) float2 cs[kGroups * D / 2];  // [token][half] cos, sin
+  after_previous();
   const int tid = threadIdx.x, lane = tid % kLanes, e0 = lane * 8;
   const int t_first = blockIdx.x * kGroups, t_last = min(t_first + kGroups, a.T) - 1;
 
@@ -235,13 +236,9 @@ int check_rope(const rnb_rope_desc* d) {
 }
 
 template <typename T>
-void launch_rope(const RopeArgs& a, int D, dim3 grid, cudaStream_t st) {
-  if (D == 64)
-    k_rope_append<T, 64><<<grid, kRopeThreads, 0, st>>>(a);
-  else if (D == 128)
-    k_rope_append<T, 128><<<grid, kRopeThreads, 0, st>>>(a);
-  else
-    k_rope_append<T, 256><<<grid, kRopeThreads, 0, st>>>(a);
+int launch_rope(const RopeArgs& a, int D, dim3 grid, cudaStream_t st) {
+  return launch("rnb_rope_append", D == 64 ? k_rope_append<T, 64> : D == 128 ? k_rope_append<T, 128> : k_rope_append<T, 256>,
+                grid, kRopeThreads, 0, st, a);
 }
 
 }  // namespace
@@ -306,9 +303,7 @@ extern "C" int rnb_rope_append(const rnb_rope_desc* d, const void* q, const void
   a.heads_a_chunk = static_cast<int>((heads + chunks - 1) / chunks);
   const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(a.T) + groups - 1) / groups),
                   static_cast<unsigned>((heads + a.heads_a_chunk - 1) / a.heads_a_chunk));
-  if (d->dtype == RNB_DTYPE_BF16)
-    launch_rope<__nv_bfloat16>(a, static_cast<int>(D), grid, static_cast<cudaStream_t>(stream));
-  else
-    launch_rope<__half>(a, static_cast<int>(D), grid, static_cast<cudaStream_t>(stream));
-  return launch_status("rnb_rope_append");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return d->dtype == RNB_DTYPE_BF16 ? launch_rope<__nv_bfloat16>(a, static_cast<int>(D), grid, st)
+                                    : launch_rope<__half>(a, static_cast<int>(D), grid, st);
 }
