@@ -655,7 +655,14 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
 struct Plan {
   int R, grid, rows;  // rows a tile, CTAs, rows that a tile can have in use
   size_t ml_off, o_off, bytes;
+  bool many;       // the many-row kernel may have work
+  AttnArgs split;  // its split of tiles (the fields that plan_split sets)
 };
+
+int max_kv_of(const rnb_attn_desc* d, const rnb_kv_cache* c) {
+  const int64_t kv = static_cast<int64_t>(d->table_cols) * c->page_size;
+  return static_cast<int>(kv < INT32_MAX - 4096 ? kv : INT32_MAX - 4096);  // steps ahead stay in 31 bits
+}
 
 Plan plan_of(const rnb_attn_desc* d, const rnb_kv_cache* c, int sms, bool cu_given) {
   Plan p;
@@ -670,6 +677,16 @@ Plan plan_of(const rnb_attn_desc* d, const rnb_kv_cache* c, int sms, bool cu_giv
   p.ml_off = (sizeof(Begun) * p.grid + 255) & ~size_t(255);
   p.o_off = (p.ml_off + 2u * p.grid * p.R * 2 * sizeof(float) + 255) & ~size_t(255);
   p.bytes = p.o_off + 2u * p.grid * p.R * static_cast<size_t>(c->head_dim) * sizeof(float);
+  p.many = cu_given && (d->max_q > 0 ? d->max_q : d->T) * group >= kManyRows;
+  p.split = AttnArgs{};
+  if (p.many) {
+    // (the two kernels' parts follow each other in one workspace)
+    size_t bytes = 0;
+    p.split.T = d->T, p.split.B = d->B, p.split.Hkv = c->n_kv_heads, p.split.group = static_cast<int>(group);
+    p.split.max_kv = max_kv_of(d, c);
+    plan_split(&p.split, c->head_dim, sms, &bytes);
+    if (bytes > p.bytes) p.bytes = bytes;
+  }
   return p;
 }
 
@@ -758,8 +775,7 @@ int rnb_paged_attention(const rnb_attn_desc* d, const rnb_kv_cache* cache, const
   a.Hq = d->n_q_heads, a.Hkv = cache->n_kv_heads, a.group = a.Hq / a.Hkv;
   while ((1 << a.log2p) < cache->page_size) ++a.log2p;
   a.num_pages = cache->num_pages;
-  const int64_t kv = static_cast<int64_t>(d->table_cols) * cache->page_size;
-  a.max_kv = static_cast<int>(kv < INT32_MAX - 4096 ? kv : INT32_MAX - 4096);  // steps ahead stay in 31 bits
+  a.max_kv = max_kv_of(d, cache);
   a.window = d->window < a.max_kv ? d->window : 0;
   a.few_rows = INT32_MAX;
   a.scale_log2 = d->scale * 1.4426950408889634f;
@@ -770,13 +786,14 @@ int rnb_paged_attention(const rnb_attn_desc* d, const rnb_kv_cache* cache, const
   // and values, so longer ones are split; at this border (224 positions of 256, 448 of
   // 128) both take the same.
   a.direct = !cu_q && static_cast<int64_t>(a.max_kv) * cache->head_dim <= 224 * 256;
-  const int64_t most = cu_q ? (d->max_q > 0 ? d->max_q : d->T) : 1;
-  if (cu_q && most * a.group >= kManyRows) {
+  if (p.many) {
     PromptMaps maps;
     if (prepare_prompt(a, cache, &maps)) {
       // (a single request is wholly the many-row kernel's, however few its rows are)
       a.few_rows = d->B == 1 ? 1 : kManyRows;
-      if ((rc = run_prompt(a, cache, maps, st))) return rc;
+      AttnArgs m = a;
+      m.split = p.split.split, m.ml_off = p.split.ml_off, m.o_off = p.split.o_off;
+      if ((rc = run_prompt(m, cache, maps, st))) return rc;
       if (d->B == 1) return RNB_OK;
     }
   }

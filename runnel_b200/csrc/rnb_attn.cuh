@@ -19,6 +19,7 @@ struct AttnArgs {
   float scale_log2;  // scale * log2(e): softmax in powers of two
   int B, T, W, Hq, Hkv, group, log2p, num_pages, window, max_kv;
   int direct;    // few-row kernel: whole tiles by number (one row a request)
+  int split;     // many-row kernel: CTAs over which the tiles' positions are split (0: not)
   int few_rows;  // requests with rows * group below this are the few-row kernel's
 };
 
@@ -30,6 +31,7 @@ struct PromptMaps {
   int k_box, v_box;  // cache rows a copy
   int tokens;        // tokens a row tile
 };
+int plan_split(AttnArgs* a, int D, int sms, size_t* bytes);
 bool prepare_prompt(const AttnArgs& a, const rnb_kv_cache* c, PromptMaps* p);
 int run_prompt(const AttnArgs& a, const rnb_kv_cache* c, const PromptMaps& p, cudaStream_t st);
 

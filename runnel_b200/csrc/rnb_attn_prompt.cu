@@ -24,6 +24,10 @@
 //   units, K as the K-major and V as the MN-major operand, both as they lie in the
 //   cache.  Pages behind the request's end (and ids out of range) are fetched at
 //   a page coordinate behind the cache, which reads as zeros.
+// * Where a call has so few tiles that SMs would stay idle (a few drafted tokens
+//   of large groups, a prompt's end on a long cache), the positions of a tile are split
+//   over CTAs: each leaves its (m, l, O) in the workspace and k_attn_join_tiles adds
+//   a tile's parts in order.
 // * Every wait is bounded; one that gives up ends the CTA with RNB_STATUS_TIMEOUT.
 //
 // The tensor cores bound it for head_dim 256 (4 D flops a row and position
@@ -204,6 +208,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return y;
 }
 
+// A tile whose positions are split, for the join.
+struct SplitTile {
+  int parts;  // 0: no tile, or one that its CTA wrote
+  int n;      // tiles of the call: part p is CTA p n + i's
+  int q0, tok0, rows, h;
+};
+
 struct Bars {
   uint64_t full[10], empty[10];   // ring units
   uint64_t q_full;              // Q in shared memory
@@ -233,9 +244,12 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
   const int tt = maps.tokens;            // tokens a row tile
   const int cta_tokens = tt * C::NQ;
 
-  // ---- which request and tokens: tiles of a request from its end (the longest first)
-  const int h = blockIdx.x % a.Hkv;
-  const int64_t want = blockIdx.x / a.Hkv;
+  // ---- which request and tokens: tiles of a request from its end (the longest first).
+  // With a.split the grid's CTAs are dealt to the call's N tiles, the i-th of each N
+  // to a tile's i-th part.
+  SplitTile* split = reinterpret_cast<SplitTile*>(a.ws);
+  int h = blockIdx.x % a.Hkv, part = 0, parts = 1, n_tiles = 0;
+  int64_t want = blockIdx.x / a.Hkv;
   {
     if (tid == 0) {
       found[0] = -1;
@@ -263,6 +277,17 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     __syncthreads();
     int64_t base = inc - sum;
     for (int w = 0; w < warp; ++w) base += wsum[w];
+    if (a.split) {
+      int64_t all = 0;
+      for (int w = 0; w < C::kThreads / 32; ++w) all += wsum[w];
+      n_tiles = static_cast<int>(all) * a.Hkv;  // at most the grid
+      if (tid == 0) split[blockIdx.x].parts = 0;  // (until it is known)
+      if (n_tiles > 0) {
+        const int i = blockIdx.x % n_tiles;
+        part = blockIdx.x / n_tiles, parts = gridDim.x / n_tiles;
+        h = i % a.Hkv, want = part < parts ? i / a.Hkv : -1;
+      }
+    }
     if (want >= base && want < base + sum) {
       int64_t rem = want - base;
       int b = lo;
@@ -284,8 +309,22 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
   const int first_p = p0 + tok0, last_p = p0 + tok_end - 1;
   const int any_lo = a.window > 0 ? max(first_p - a.window + 1, 0) : 0;
   const int kv_end = max(last_p + 1, 0);
-  const int blk0 = any_lo / C::BN;
-  const int nblk = max((kv_end + C::BN - 1) / C::BN - blk0, 0);
+  int blk0 = any_lo / C::BN;
+  int nblk = max((kv_end + C::BN - 1) / C::BN - blk0, 0);
+  if (a.split) {
+    // (two blocks a part or more: a part's start and end cost about two)
+    parts = max(min(parts, nblk / 2), 1);
+    if (tid == 0 && part == 0 && parts > 1) {
+      SplitTile t;
+      t.parts = parts, t.n = n_tiles;
+      t.q0 = q0, t.tok0 = tok0, t.rows = rows, t.h = h;
+      split[blockIdx.x] = t;
+    }
+    if (part >= parts) return;
+    const int lo = static_cast<int>(static_cast<int64_t>(nblk) * part / parts);
+    nblk = static_cast<int>(static_cast<int64_t>(nblk) * (part + 1) / parts) - lo;
+    blk0 += lo;
+  }
   const int32_t* row_table = a.table + static_cast<int64_t>(b) * a.W;
   // a row tile in shared memory: 64-element columns of 128 rows, 128-byte swizzle
   constexpr int kCol = 128 * 128;
@@ -385,11 +424,12 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
         next = ahead;
       }
     }
-    if (a.gate && alive && nblk > 0) alive = wait_on(&bars.q_done, 0);
-    if (a.gate && alive) load_tiles(&maps.gate, &bars.g_full);
+    const bool gates = a.gate && parts == 1;
+    if (gates && alive && nblk > 0) alive = wait_on(&bars.q_done, 0);
+    if (gates && alive) load_tiles(&maps.gate, &bars.g_full);
     // no copy may be in flight when the CTA ends
     if (nblk > 0) wait_on(&bars.q_full, 0);
-    if (a.gate && alive) wait_on(&bars.g_full, 0);
+    if (gates && alive) wait_on(&bars.g_full, 0);
     for (int v = max(u - C::NST, 0); v < u; ++v) wait_on(&bars.full[v % C::NST], (v / C::NST) & 1);
   } else if (warp == 1) {
     // ---- issuer
@@ -596,8 +636,29 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
     // parity only tells neighbouring phases apart)
     if (alive && nblk > 0) alive = wait_on(&bars.o_last[wg], 0);
     tc_fence_after();
-    if (a.gate && alive) alive = wait_on(&bars.g_full, 0);
-    if (alive) {
+    if (parts > 1) {
+      // this part's row of O, m and l for the join
+      const int64_t row = (static_cast<int64_t>(blockIdx.x) * C::NQ + wg) * 128 + r;
+      float* po = reinterpret_cast<float*>(a.ws + a.o_off) + row * D;
+      if (in && alive) {
+        float* ml = reinterpret_cast<float*>(a.ws + a.ml_off) + 2 * row;
+        ml[0] = m, ml[1] = l;
+      }
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32(t_o + 32 * c, o);
+        tmem_wait_ld();
+        if (in && alive) {
+#pragma unroll
+          for (int x = 0; x < 8; ++x)
+            *reinterpret_cast<uint4*>(po + 32 * c + 4 * x) = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+        }
+      }
+    }
+    const bool whole = alive && parts == 1;
+    if (a.gate && whole) alive = wait_on(&bars.g_full, 0);
+    if (whole && alive) {
       // in place of Q, or of the gates that have come there
       char* base = smem + wg * (D / 64) * kCol;
       const float inv = l > 0.f ? 1.0f / l : 0.f;
@@ -635,7 +696,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
       fence_proxy_async_smem();
     }
     // the warpgroup's four warps, those that gave up among them
-    if (all_of_128(1 + wg, alive)) {
+    if (all_of_128(1 + wg, whole && alive)) {
       const char* base = smem + wg * (D / 64) * kCol;
       if (wt0 + tt <= rows) {
         if (r == 0) {
@@ -662,17 +723,64 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
   if (warp == 2) tmem_dealloc(tmem, 512);
 }
 
+// Block (i, y): rows [16 y, 16 y + 16) of split tile i.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) k_attn_join_tiles(const AttnArgs a, int tokens) {
+  after_previous();
+  using C = Cfg<D>;
+  constexpr int kCols = D / 4, kRowsIt = 256 / kCols;
+  const SplitTile* split = reinterpret_cast<const SplitTile*>(a.ws);
+  const SplitTile tile = split[blockIdx.x];
+  if (tile.parts < 2) return;
+  const int col = threadIdx.x % kCols;
+  for (int x = threadIdx.x / kCols; x < 16; x += kRowsIt) {
+    const int rr = blockIdx.y * 16 + x, q = rr / 128, r = rr - 128 * q;
+    const int tok = tile.tok0 + q * tokens + r / a.group, head = tile.h * a.group + r % a.group;
+    if (r >= tokens * a.group || tok >= tile.rows) continue;
+    const uint2 gw = a.gate ? __ldg(reinterpret_cast<const uint2*>(attn_gate<T>(a, tile.q0 + tok, head) + 4 * col))
+                            : make_uint2(0, 0);
+    const float* ml = reinterpret_cast<const float*>(a.ws + a.ml_off);
+    const float* po = reinterpret_cast<const float*>(a.ws + a.o_off);
+    auto row_of = [&](int p) {
+      return (static_cast<int64_t>(p * tile.n + static_cast<int>(blockIdx.x)) * C::NQ + q) * 128 + r;
+    };
+    float mx = -INFINITY;
+    for (int p = 0; p < tile.parts; ++p) mx = fmaxf(mx, ml[2 * row_of(p)]);
+    const float use = mx == -INFINITY ? 0.f : mx;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+#pragma unroll 4
+    for (int p = 0; p < tile.parts; ++p) {
+      const int64_t row = row_of(p);
+      const float f = ex2(ml[2 * row] - use);
+      const float4 v = *reinterpret_cast<const float4*>(po + row * D + 4 * col);
+      acc.x = fmaf(v.x, f, acc.x), acc.y = fmaf(v.y, f, acc.y);
+      acc.z = fmaf(v.z, f, acc.z), acc.w = fmaf(v.w, f, acc.w);
+      l = fmaf(ml[2 * row + 1], f, l);
+    }
+    attn_write_row<T, D>(a, tile.q0 + tok, head, 4 * col, acc, mx, l, gw);
+  }
+}
+
+template <int D>
+int64_t tiles_at_most(const AttnArgs& a) {
+  const int64_t per = static_cast<int64_t>(128 / a.group) * Cfg<D>::NQ;  // tokens a CTA
+  return (a.T + per - 1) / per + (a.B < a.T ? a.B : a.T);
+}
+
 template <typename T, int D>
 int launch_prompt(const AttnArgs& a, const PromptMaps& maps, cudaStream_t st) {
   using C = Cfg<D>;
   const cudaError_t e = cudaFuncSetAttribute(k_attn_prompt<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (e != cudaSuccess) return fail(RNB_ERR_CUDA, std::string("rnb_paged_attention: ") + cudaGetErrorString(e));
   // as many tiles as there can be: CTAs without one end at once
-  const int64_t per = static_cast<int64_t>(maps.tokens) * C::NQ;
-  const int64_t tiles = (a.T + per - 1) / per + (a.B < a.T ? a.B : a.T);
-  if (tiles * a.Hkv > INT32_MAX) return fail(RNB_ERR_INVALID, "rnb_paged_attention: too many rows");
-  return launch("rnb_paged_attention", k_attn_prompt<T, D>, static_cast<unsigned>(tiles * a.Hkv), C::kThreads, C::kSmem, st,
-                a, maps);
+  const int64_t ctas = tiles_at_most<D>(a) * a.Hkv;
+  if (ctas > INT32_MAX) return fail(RNB_ERR_INVALID, "rnb_paged_attention: too many rows");
+  const unsigned grid = static_cast<unsigned>(a.split ? a.split : ctas);
+  const int rc = launch("rnb_paged_attention", k_attn_prompt<T, D>, grid, C::kThreads, C::kSmem, st, a, maps);
+  if (rc || !a.split) return rc;
+  return launch("rnb_paged_attention join", k_attn_join_tiles<T, D>, dim3(static_cast<unsigned>(ctas), C::NQ * 128 / 16),
+                256, 0, st, a, maps.tokens);
 }
 
 bool encode_cache(CUtensorMap* m, const rnb_kv_cache* c, const void* base, int64_t page_stride, int64_t head_stride,
@@ -713,6 +821,22 @@ bool prepare_prompt(const AttnArgs& a, const rnb_kv_cache* c, PromptMaps* p) {
          encode_rows(&p->q, a, a.q, D, a.q_ts, a.q_hs, p->tokens) &&
          encode_rows(&p->out, a, a.out, D, static_cast<int64_t>(a.Hq) * D, D, p->tokens) &&
          (!a.gate || encode_rows(&p->gate, a, a.gate, D, a.g_ts, a.g_hs, p->tokens));
+}
+
+// CTAs of a call whose tiles are split (0: not split), and its workspace: where
+// the tiles that there can be do not fill the SMs, and are long enough.
+int plan_split(AttnArgs* a, int D, int sms, size_t* bytes) {
+  a->split = 0;
+  *bytes = 0;
+  if (a->group > 128 || a->max_kv < 4 * Cfg<128>::BN) return 0;
+  const int64_t tiles = D == 256 ? tiles_at_most<256>(*a) : D == 128 ? tiles_at_most<128>(*a) : tiles_at_most<64>(*a);
+  if (tiles * a->Hkv > sms) return 0;
+  const size_t rows = static_cast<size_t>(sms) * (D == 256 ? 1 : 2) * 128;
+  a->split = sms;
+  a->ml_off = (sizeof(SplitTile) * sms + 255) & ~size_t(255);
+  a->o_off = a->ml_off + 2 * sizeof(float) * rows;
+  *bytes = a->o_off + sizeof(float) * rows * D;
+  return a->split;
 }
 
 int run_prompt(const AttnArgs& a, const rnb_kv_cache* c, const PromptMaps& p, cudaStream_t st) {

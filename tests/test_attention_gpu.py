@@ -361,6 +361,23 @@ def test_prompts(Hq, Hkv, D, dtype):
     _check_attention(q, kc, vc, table, lens, rows, gate=gate)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("Hq,Hkv,D,lens,rows", [
+    (12, 1, 128, [9000, 300, 4097, 1], [7, 7, 6, 1]), (16, 2, 256, [5000], [40]), (40, 2, 64, [3001, 2500], [9, 200]),
+    (12, 1, 256, [2000, 0, 1500], [20, 0, 7]), (100, 1, 128, [1300, 700], [1, 3]),
+])
+def test_few_tiles_over_long_caches(dtype, Hq, Hkv, D, lens, rows):
+    """Tiles whose positions are split over CTAs and joined, single rows among them, windows and gates too."""
+    g = _gen(sum(lens))
+    kc, vc, table = _cache_of(g, dtype, lens, Hkv, D, 16 if D == 64 else 64)
+    q = _rand(g, dtype, sum(rows), Hq, D, scale=1.5)
+    gate = _rand(g, dtype, sum(rows), Hq, D)
+    _check_attention(q, kc, vc, table, lens, rows, max_q=max(rows), cu=_i([0, *itertools.accumulate(rows)]))
+    _check_attention(q, kc, vc, table, lens, rows, cu=_i([0, *itertools.accumulate(rows)]), gate=gate)
+    _check_attention(q, kc, vc, table, lens, rows, cu=_i([0, *itertools.accumulate(rows)]), gate=gate, window=1000)
+    assert attention.status() == 0
+
+
 @pytest.mark.parametrize("n,r", [(1, 1), (70, 1), (300, 3), (40, 64), (257, 200), (0, 5), (130, 0)])
 @pytest.mark.parametrize("Hq,Hkv,D", [(16, 2, 256), (7, 1, 128), (64, 1, 64), (200, 1, 64)])
 def test_a_single_request_of_any_rows(n, r, Hq, Hkv, D):
