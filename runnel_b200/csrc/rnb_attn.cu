@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
   int s = 0, s_end = 0;  // positions: the step whose K and V are (being) loaded, the segment's end
   const int pmask = (1 << a.log2p) - 1;
   auto positions_end = [&](const Segment& sg) {
-    const int last = sg.len - sg.rows + min(sg.tile * R + R - 1, sg.rows * a.group - 1) / a.group;
+    const int last = sg.len - sg.rows + by_group(a, min(sg.tile * R + R - 1, sg.rows * a.group - 1));
     return min((sg.blk0 + sg.blk + sg.n) * kUnit, last + 1);
   };
   auto enter = [&](const Segment& sg) {
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
   auto load_q = [&](const Segment& sg, int buf) {
     constexpr int kPer = D / 8;
     for (int x = tid; x < R * kPer; x += kThreads) {
-      const int r = x / kPer, e = (x - r * kPer) * 8, row = sg.tile * R + r, i = row / a.group, j = row - i * a.group;
+      const int r = x / kPer, e = (x - r * kPer) * 8, row = sg.tile * R + r, i = by_group(a, row), j = row - i * a.group;
       if (row < sg.rows * a.group)
         cp_async16(&sm.q[buf][r][e],
                    static_cast<const T*>(a.q) + (sg.q0 + i) * a.q_ts + (sg.h * a.group + j) * a.q_hs + e);
@@ -354,11 +354,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int row = min(row0 + nt * 8 + 2 * c + e, work - 1), p = p0 + row / a.group;
+        const int row = min(row0 + nt * 8 + 2 * c + e, work - 1), p = p0 + by_group(a, row);
         seen_hi[nt][e] = p;
         seen_lo[nt][e] = a.window > 0 ? p - a.window + 1 : INT_MIN;
       }
-    const int first_p = p0 + row0 / a.group, last_p = p0 + min(row0 + R - 1, work - 1) / a.group;
+    const int first_p = p0 + by_group(a, row0), last_p = p0 + by_group(a, min(row0 + R - 1, work - 1));
     const int all_lo = a.window > 0 ? last_p - a.window + 1 : INT_MIN;   // from here every row sees, up to first_p
     const int any_lo = a.window > 0 ? first_p - a.window + 1 : INT_MIN;  // before here none does
 
@@ -548,41 +548,53 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
     const int part = 2 * blockIdx.x + (begins ? 1 : 0);
     float* part_ml = reinterpret_cast<float*>(a.ws + a.ml_off) + static_cast<int64_t>(part) * R * 2;
     float* part_o = reinterpret_cast<float*>(a.ws + a.o_off) + static_cast<int64_t>(part) * R * D;
-    constexpr int kPieces = R * (D / 4) / kThreads;  // of four elements, a thread
+    // a thread has kPieces pieces of four elements of one row
+    constexpr int kLanes = kThreads / R, kPieces = D / 4 / kLanes;
     const bool done = begins && ends;
-    uint2 gw[kPieces];
-    if (done && a.gate) {  // all under way at once
+    const int r = tid / kLanes, d0 = (tid % kLanes) * 4, row = row0 + r;
+    if (row < work) {
+      const int i = by_group(a, row), t = sg.q0 + i, head = sg.h * a.group + row - i * a.group;
+      uint2 gw[kPieces];
+      if (done && a.gate) {
 #pragma unroll
-      for (int y = 0; y < kPieces; ++y) {
-        const int z = y * kThreads + tid, r = z / (D / 4), row = row0 + r;
-        if (row < work)
-          gw[y] = __ldg(reinterpret_cast<const uint2*>(attn_gate<T>(a, sg.q0 + row / a.group, sg.h * a.group + row % a.group) +
-                                                       (z - r * (D / 4)) * 4));
+        for (int y = 0; y < kPieces; ++y)
+          gw[y] = __ldg(reinterpret_cast<const uint2*>(attn_gate<T>(a, t, head) + d0 + 4 * kLanes * y));
       }
-    }
-#pragma unroll
-    for (int y = 0; y < kPieces; ++y) {
-      const int z = y * kThreads + tid, r = z / (D / 4), d = (z - r * (D / 4)) * 4, row = row0 + r;
-      if (row >= work) break;  // (rows ascend)
       float mx = sm.m[0][r];
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) mx = fmaxf(mx, sm.m[w][r]);
       const float use = mx == -INFINITY ? 0.f : mx;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      float ls = 0.f;
+      float wf[kWarps], ls = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float wf = ex2(sm.m[w][r] - use);
-        const float4 v = *reinterpret_cast<const float4*>(&sm.o[w][r][d]);
-        acc.x = fmaf(v.x, wf, acc.x), acc.y = fmaf(v.y, wf, acc.y);
-        acc.z = fmaf(v.z, wf, acc.z), acc.w = fmaf(v.w, wf, acc.w);
-        ls = fmaf(sm.l[w][r], wf, ls);
+        wf[w] = ex2(sm.m[w][r] - use);
+        ls = fmaf(sm.l[w][r], wf[w], ls);
+      }
+      if (d0 == 0) {
+        if (done)
+          attn_write_lse(a, t, head, mx, ls);
+        else
+          part_ml[2 * r] = mx, part_ml[2 * r + 1] = ls;
       }
       if (done) {
-        attn_write_row<T, D>(a, sg.q0 + row / a.group, sg.h * a.group + row % a.group, d, acc, mx, ls, gw[y]);
-      } else {
-        *reinterpret_cast<float4*>(part_o + r * D + d) = acc;
-        if (d == 0) part_ml[2 * r] = mx, part_ml[2 * r + 1] = ls;
+        const float inv = ls > 0.f ? 1.0f / ls : 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) wf[w] *= inv;
+      }
+#pragma unroll
+      for (int y = 0; y < kPieces; ++y) {
+        const int d = d0 + 4 * kLanes * y;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float4 v = *reinterpret_cast<const float4*>(&sm.o[w][r][d]);
+          acc.x = fmaf(v.x, wf[w], acc.x), acc.y = fmaf(v.y, wf[w], acc.y);
+          acc.z = fmaf(v.z, wf[w], acc.z), acc.w = fmaf(v.w, wf[w], acc.w);
+        }
+        if (done)
+          attn_write_four<T, D>(a, t, head, d, acc, gw[y]);
+        else
+          *reinterpret_cast<float4*>(part_o + r * D + d) = acc;
       }
     }
     if (begins && !ends && tid == 0) {
@@ -613,7 +625,7 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
   const float* po = reinterpret_cast<const float*>(a.ws + a.o_off);
   auto part = [&](int i) { return static_cast<int64_t>(2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * R + r; };
   const int col = tid % kCols, way = tid / kCols;
-  const int t = bg.q0 + row / a.group, head = bg.h * a.group + row % a.group;
+  const int i = by_group(a, row), t = bg.q0 + i, head = bg.h * a.group + row - i * a.group;
   uint2 gw = make_uint2(0, 0);
   if (a.gate && way == 0) gw = __ldg(reinterpret_cast<const uint2*>(attn_gate<T>(a, t, head) + 4 * col));
   float mx = -INFINITY;
@@ -772,7 +784,8 @@ int rnb_paged_attention(const rnb_attn_desc* d, const rnb_kv_cache* cache, const
   a.kc_ps = cache->k_page_stride, a.kc_hs = cache->k_head_stride;
   a.vc_ps = cache->v_page_stride, a.vc_hs = cache->v_head_stride;
   a.B = d->B, a.T = d->T, a.W = d->table_cols;
-  a.Hq = d->n_q_heads, a.Hkv = cache->n_kv_heads, a.group = a.Hq / a.Hkv;
+  a.Hq = d->n_q_heads, a.Hkv = cache->n_kv_heads;
+  set_group(&a, a.Hq / a.Hkv);
   while ((1 << a.log2p) < cache->page_size) ++a.log2p;
   a.num_pages = cache->num_pages;
   a.max_kv = max_kv_of(d, cache);
