@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
   Begun* begun = reinterpret_cast<Begun*>(a.ws);
   if (tid == 0) begun[blockIdx.x].last = -1;
 
-  // ---- this CTA's share.  The thread whose requests hold its first unit deals the
+  // ---- this CTA's share.  The warp whose requests hold its first unit deals the
   // segments from there, two ahead of the one in work: it stands at cost p_at of row
   // tile tile_at of key head h_at of request `at`, whose numbers are c0, c1, len.
   bool dealer = false;
@@ -179,14 +179,22 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
     if (tid == kThreads - 1) total = base + sum;
     __syncthreads();
     const int64_t share = share_of(total, gridDim.x), u0 = share * blockIdx.x;
-    if (u0 >= base && u0 < base + sum) {
-      dealer = true;
+    const bool here = u0 >= base && u0 < base + sum;
+    if (here) {
       start_rem = u0 - base;
       at = lo;
       for (int64_t n = per == 1 ? sum : units(at); start_rem >= n && at + 1 < hi; n = units(at)) {
         start_rem -= n;
         ++at;
       }
+    }
+    const uint32_t who = __ballot_sync(0xffffffffu, here);
+    dealer = who != 0;
+    if (dealer) {
+      const int from = __ffs(who) - 1;
+      start_rem = __shfl_sync(0xffffffffu, start_rem, from), at = __shfl_sync(0xffffffffu, at, from);
+      c0 = __shfl_sync(0xffffffffu, c0, from), c1 = __shfl_sync(0xffffffffu, c1, from);
+      len = __shfl_sync(0xffffffffu, len, from);
     }
   }
   // (direct: every request has one row, so tile i is known without the lengths;
@@ -198,6 +206,19 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
   if (u0 >= u1) return;
 
   int64_t u_at = u0;
+  // From an idle request to the next one that has tiles here: 32 are read at once, so
+  // that a batch's empty places cost little (4092 of 4096 places idle: 331 -> 68 us).
+  auto skip_idle = [&]() {
+    for (uint32_t live = 0; live == 0 && at < a.B;) {
+      const int left = a.B - 1 - at;
+      read_request(a, lane < left ? at + 1 + lane : a.B, c0, c1, len);
+      live = __ballot_sync(0xffffffffu, lane < left && request_of<R>(a, c0, c1, len).ntile > 0);
+      const int i = live ? __ffs(live) - 1 : min(left, 31);
+      at += i + 1;  // (nothing left: B)
+      c0 = __shfl_sync(0xffffffffu, c0, i), c1 = __shfl_sync(0xffffffffu, c1, i);
+      len = __shfl_sync(0xffffffffu, len, i);
+    }
+  };
   auto deal = [&](Segment& sg) {
     sg.n = 0;
     if (a.direct) {
@@ -230,7 +251,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
           if (++tile_at == rq.ntile) tile_at = 0, ++h_at;
         }
       }
-      if (h_at == a.Hkv || rq.ntile == 0) {  // the next request's numbers are on their way when they are asked for
+      if (rq.ntile == 0) {
+        skip_idle();
+        h_at = tile_at = p_at = 0;
+      } else if (h_at == a.Hkv) {  // the next request's numbers are on their way when they are asked for
         h_at = tile_at = p_at = 0;
         read_request(a, ++at, c0, c1, len);
       }
@@ -238,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
     }
   };
   if (a.direct) {
-    dealer = tid == 0;
+    dealer = warp == 0;
     if (dealer) {
       deal(sm.seg[0]);
       deal(sm.seg[1]);

@@ -361,6 +361,31 @@ def test_prompts(Hq, Hkv, D, dtype):
     _check_attention(q, kc, vc, table, lens, rows, gate=gate)
 
 
+@pytest.mark.parametrize("B,active", [(33, 2), (300, 3), (3000, 5), (3000, 900)])
+@pytest.mark.parametrize("max_q", [1, 3])
+def test_idle_places_between_requests(B, active, max_q):
+    """A large batch with few requests at work, anywhere in it; the others have lengths but no rows, or nothing."""
+    g, r = _gen(B + active), random.Random(B * active)
+    rows, lens = [0] * B, [r.choice([0, 0, 40]) for _ in range(B)]
+    for b in [0, B - 1] + r.sample(range(1, B - 1), active - 2):
+        rows[b], lens[b] = r.randint(1, max_q), r.choice([1, 65, 300, 900])
+    kc, vc, table = _cache_of(g, BF16, lens, 2, 64, 16)
+    T = sum(rows)
+    q = _rand(g, BF16, T, 14, 64)
+    cu = _i([0, *itertools.accumulate(rows)])
+    out, lse = attention.paged_attention(q, kc, vc, table, _i(lens), cu_q=cu, max_q=max_q, return_lse=True)
+    few = [b for b in range(B) if rows[b]][:40]
+    n = sum(rows[b] for b in few)
+    want, wlse, tol, ltol = ref.attention(q[:n], kc, vc, table[few], [lens[b] for b in few], [rows[b] for b in few])
+    ref.close(out[:n], want, tol, "out")
+    ref.close(lse[:n], wlse, ltol, "lse")
+    last = [b for b in range(B) if rows[b]][-5:]
+    m = sum(rows[b] for b in last)
+    want, _, tol, _ = ref.attention(q[T - m:], kc, vc, table[last], [lens[b] for b in last], [rows[b] for b in last])
+    ref.close(out[T - m:], want, tol, "the last requests")
+    assert attention.status() == 0
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("Hq,Hkv,D,lens,rows", [
     (12, 1, 128, [9000, 300, 4097, 1], [7, 7, 6, 1]), (16, 2, 256, [5000], [40]), (40, 2, 64, [3001, 2500], [9, 200]),
