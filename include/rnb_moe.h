@@ -473,9 +473,9 @@ RNB_API int rnb_rope_append(const rnb_rope_desc* d, const void* q, const void* k
  * were.  Softmax statistics and sums are fp32; probabilities are rounded to
  * the cache's type for the product with V.  What lies in the cache behind a
  * request's length never counts, whatever its bits; within the length values
- * must be finite, except that a request's single row may have any bits in
- * positions that its window leaves out.  Any number of rows per request;
- * requests in any mix.  max_q (0: unknown) bounds the rows of a request and
+ * must be finite where any of the request's rows sees them: what lies before the
+ * window of its first row may have any bits, and pages wholly before it any id.
+ * Any number of rows per request; requests in any mix.  max_q (0: unknown) bounds the rows of a request and
  * only picks the kernels.  The workspace needs no initial state; calls that
  * may overlap need one each.  Results do not depend on timing: equal inputs
  * give equal bits.  A device wait inside the many-row kernel that gives up after

@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
         for (int ns = 0; ns < NS; ++ns) {
           const int st = s_cur + 16 * ns;
           const bool ok = static_cast<uint32_t>(cur[ns]) < static_cast<uint32_t>(a.num_pages);
-          if (!ok && st < seg_end && lane == 0) atomicOr(&g_attn_status, RNB_STATUS_BAD_INDEX);
+          if (!ok && st < seg_end && st + 15 >= any_lo && lane == 0) atomicOr(&g_attn_status, RNB_STATUS_BAD_INDEX);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll

@@ -444,6 +444,27 @@ def test_single_rows_ignore_any_bits_before_their_window():
     assert torch.equal(attention.paged_attention(q, kc, vc, table, _i([300]), window=37), want)
 
 
+@pytest.mark.parametrize("rows", [1, 3, 80])
+@pytest.mark.parametrize("D,Hq,Hkv,P", [(256, 16, 2, 16), (128, 32, 8, 64), (64, 4, 4, 32), (128, 4, 4, 256)])
+@pytest.mark.parametrize("window", [1, 37, 200])
+def test_positions_before_every_window_hold_any_bits(rows, D, Hq, Hkv, P, window):
+    """What no row of a request sees never counts, and its pages may be another's, or gone."""
+    g, n = _gen(8), 700
+    kc, vc, table = _cache_of(g, BF16, [n, 20], Hkv, D, P)
+    q = _rand(g, BF16, rows + 1, Hq, D)
+    args = dict(cu_q=_i([0, rows, rows + 1]), max_q=rows, window=window, return_lse=True)
+    want = attention.paged_attention(q, kc, vc, table, _i([n, 20]), **args)
+    before = n - rows - window + 1
+    for j in range(before):
+        kc[table[0, j // P], :, j % P] = float("nan")
+        vc[table[0, j // P], :, j % P] = float("inf")
+    table[0, : before // P] = -1
+    assert attention.status() == 0
+    got = attention.paged_attention(q, kc, vc, table, _i([n, 20]), **args)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert attention.status() == 0
+
+
 @pytest.mark.parametrize("D,Hq,Hkv", [(256, 16, 2), (128, 32, 8), (64, 4, 4)])
 def test_large_scores_and_scales(D, Hq, Hkv):
     """Peaked softmax, its maximum late, and a scale that is not the default."""
