@@ -475,12 +475,13 @@ RNB_API int rnb_rope_append(const rnb_rope_desc* d, const void* q, const void* k
  * request's length never counts, whatever its bits; within the length values
  * must be finite where any of the request's rows sees them: what lies before the
  * window of its first row may have any bits, and pages wholly before it any id.
- * Any number of rows per request; requests in any mix.  max_q (0: unknown) bounds the rows of a request and
- * only picks the kernels.  The workspace needs no initial state; calls that
- * may overlap need one each.  Results do not depend on timing: equal inputs
- * give equal bits.  A device wait inside the many-row kernel that gives up after
- * a second sets RNB_STATUS_TIMEOUT: results are void then, and until the status
- * is read many-row requests are left out. */
+ * Any number of rows per request; requests in any mix.  out may be q where q is
+ * packed; otherwise it shares no memory with q or gate.  max_q (0: unknown)
+ * bounds the rows of a request and only picks the kernels.  The workspace needs
+ * no initial state; calls that may overlap need one each.  Results do not depend
+ * on timing: equal inputs give equal bits.  A device wait inside the many-row
+ * kernel that gives up after a second sets RNB_STATUS_TIMEOUT: results are void
+ * then, and until the status is read many-row requests are left out. */
 typedef struct rnb_attn_desc {
   int32_t B;
   int32_t T;          /* rows of q and out */

@@ -116,7 +116,8 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     ``positions`` is ``[axes, T]`` (or ``[T]``: all axes alike); ``sections`` says how many
     frequencies each axis (for images: time, height, width) turns, one section
     after the other, or in turns with ``interleaved``.  Rows with slot -1 are
-    left alone, in ``out`` too.  ``out`` may be ``q`` if that is contiguous.
+    left alone, in ``out`` too; the other slots are distinct (of two tokens in one,
+    either may stay).  ``out`` may be ``q`` if that is contiguous.
     """
     if k_cache is None or slots is None:
         raise ValueError("rope_append needs a cache and slots; rope() turns queries without them")
@@ -143,7 +144,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     it (``window`` > 0: its last ``window`` positions only).  ``scale`` defaults to
     ``head_dim ** -0.5``; with ``gate`` ``[T, Hq, D]`` the output is multiplied by its
     sigmoid.  A row that sees nothing gives zeros and lse -inf.  Rows of ``out``
-    behind ``cu_q[-1]`` are left as they were.  ``max_q``, a bound on the rows of one
+    behind ``cu_q[-1]`` are left as they were.  ``out`` may be ``q`` if that is contiguous,
+    but not share memory with it otherwise, nor with ``gate``.  ``max_q``, a bound on the rows of one
     request, picks the kernels and is worth giving.
     """
     return (_calls or _native()).paged_attention(q, k_cache, v_cache, table, seq_lens, cu_q, max_q, scale, window, gate, out,

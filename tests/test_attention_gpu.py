@@ -444,6 +444,24 @@ def test_single_rows_ignore_any_bits_before_their_window():
     assert torch.equal(attention.paged_attention(q, kc, vc, table, _i([300]), window=37), want)
 
 
+@pytest.mark.parametrize("lens,rows", [([300, 70, 9000], [1, 1, 1]), ([300, 70, 9000], [3, 2, 4]),
+                                       ([300, 150, 700], [1, 150, 130]), ([5000], [70])])
+@pytest.mark.parametrize("Hq,Hkv,D", [(16, 2, 256), (28, 4, 128), (4, 4, 64)])
+def test_outputs_in_place(lens, rows, Hq, Hkv, D):
+    g = _gen(31)
+    kc, vc, table = _cache_of(g, BF16, lens, Hkv, D, 16)
+    q, gate = _rand(g, BF16, sum(rows), Hq, D), _rand(g, BF16, sum(rows), Hq, D)
+    cu = None if rows == [1] * len(rows) else _i([0, *itertools.accumulate(rows)])
+    for gt in (None, gate):
+        args = dict(cu_q=cu, max_q=max(rows))
+        want = attention.paged_attention(q, kc, vc, table, _i(lens), gate=gt, **args)
+        for _ in range(5):
+            x = q.clone()
+            assert attention.paged_attention(x, kc, vc, table, _i(lens), gate=gt, out=x, **args) is x
+            assert torch.equal(x, want)
+    assert attention.status() == 0
+
+
 @pytest.mark.parametrize("rows", [1, 3, 80])
 @pytest.mark.parametrize("D,Hq,Hkv,P", [(256, 16, 2, 16), (128, 32, 8, 64), (64, 4, 4, 32), (128, 4, 4, 256)])
 @pytest.mark.parametrize("window", [1, 37, 200])
