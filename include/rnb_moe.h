@@ -417,8 +417,11 @@ RNB_API int rnb_kv_release(int B, int table_cols, int page_size, const int32_t* 
                            const int32_t* finished, int32_t* free_pages, int free_capacity,
                            const int32_t* free_count, int32_t* lens_out, int32_t* free_count_out, void* stream);
 /* Status bits (RNB_STATUS_*) of the attention-side calls on the current
- * device since the last read: copies them to *status and clears them.
- * Synchronises the stream; not for use while a stream is being captured. */
+ * device since the last read: copies them to *status and clears them, in one
+ * step on the device, so that a bit which a kernel of another stream sets
+ * meanwhile is in this read or in the next.  The bits are the device's, not a
+ * stream's: whoever reads them takes those of all callers.  Synchronises the
+ * stream; not for use while a stream is being captured. */
 RNB_API int rnb_kv_status(uint32_t* status, void* stream);
 
 /* Rotary positions with one to four axes, after an optional RMSNorm of each

@@ -89,8 +89,9 @@ def kv_release(table: torch.Tensor, lens: torch.Tensor, finished: torch.Tensor, 
 
 
 def status(device=None) -> int:
-    """Status bits (``_lib.STATUS_*``) of this module's calls on a device since
-    the last read; clears them and synchronises the current stream."""
+    """Status bits (``_lib.STATUS_*``) of this module's calls on a device, on any
+    stream, since the last read; clears them and synchronises the current stream.
+    One reader a device: it takes the bits of all callers."""
     dev = torch.device("cuda" if device is None else device)
     if dev.type != "cuda":
         raise ValueError("status is kept for CUDA devices")

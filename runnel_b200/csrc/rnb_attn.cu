@@ -764,7 +764,7 @@ int check_attn(const rnb_attn_desc* d, const rnb_kv_cache* c) {
 
 }  // namespace
 
-int attn_status_take(uint32_t* bits, cudaStream_t st) { return status_take(g_attn_status, bits, st); }
+cudaError_t attn_status_word(uint32_t** p) { return status_word(g_attn_status, p); }
 
 }  // namespace rnb
 

@@ -805,7 +805,7 @@ bool encode_rows(CUtensorMap* m, const AttnArgs& a, const void* base, int D, int
 
 }  // namespace
 
-int prompt_status_take(uint32_t* bits, cudaStream_t st) { return status_take(g_prompt_status, bits, st); }
+cudaError_t prompt_status_word(uint32_t** p) { return status_word(g_prompt_status, p); }
 
 bool prepare_prompt(const AttnArgs& a, const rnb_kv_cache* c, PromptMaps* p) {
   if (a.group > 128) return false;

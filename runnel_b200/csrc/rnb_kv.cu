@@ -18,6 +18,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <mutex>
 #include <string>
 
 #include "rnb_kv.cuh"
@@ -29,6 +30,21 @@ constexpr int kPlanThreads = 256;
 constexpr int kPlanMaxB = 16384;
 
 __device__ uint32_t g_kv_status;
+
+// The words are shared by all streams of the device, and a kernel may set a bit
+// at any time: each is exchanged for zero, so that every bit is either in this
+// read or in the next.
+__device__ uint32_t g_status_taken;
+
+struct StatusWords {
+  uint32_t* word[4];
+};
+
+__global__ void k_take_status(const StatusWords s) {
+  uint32_t bits = 0;
+  for (uint32_t* w : s.word) bits |= atomicExch(w, 0u);
+  g_status_taken = bits;
+}
 
 // Exclusive sums, in place, over n values of two shared arrays (values >= 0,
 // sums saturating at 2^31 - 1); totals in tot[0..1].  Every thread of the
@@ -286,12 +302,22 @@ int rnb_kv_status(uint32_t* status, void* stream) {
   int rc = check_device();
   if (rc) return rc;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  uint32_t v[4] = {0, 0, 0, 0};
-  if ((rc = status_take(g_kv_status, &v[0], st))) return rc;
-  if ((rc = rope_status_take(&v[1], st))) return rc;
-  if ((rc = attn_status_take(&v[2], st))) return rc;
-  if ((rc = prompt_status_take(&v[3], st))) return rc;
-  *status = v[0] | v[1] | v[2] | v[3];
+  static std::mutex one_reader;  // g_status_taken is one word
+  const std::lock_guard<std::mutex> lock(one_reader);
+  StatusWords words{};
+  cudaError_t e = status_word(g_kv_status, &words.word[0]);
+  if (e == cudaSuccess) e = rope_status_word(&words.word[1]);
+  if (e == cudaSuccess) e = attn_status_word(&words.word[2]);
+  if (e == cudaSuccess) e = prompt_status_word(&words.word[3]);
+  if (e == cudaSuccess) {
+    k_take_status<<<1, 1, 0, st>>>(words);
+    e = cudaGetLastError();
+  }
+  uint32_t bits = 0;
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbolAsync(&bits, g_status_taken, sizeof bits, 0, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e != cudaSuccess) return fail(RNB_ERR_CUDA, std::string("rnb_kv_status: ") + cudaGetErrorString(e));
+  *status = bits;
   return RNB_OK;
 }
 

@@ -68,20 +68,15 @@ __device__ __forceinline__ void after_previous() {
   griddep_launch_dependents();
 }
 
-// Reads and clears one unit's device status word (synchronises the stream).
-int rope_status_take(uint32_t* bits, cudaStream_t st);
-int attn_status_take(uint32_t* bits, cudaStream_t st);
-int prompt_status_take(uint32_t* bits, cudaStream_t st);
+// The address on the current device of each unit's status word, which its kernels
+// set bits of (atomicOr) and rnb_kv_status takes.
+cudaError_t rope_status_word(uint32_t** p);
+cudaError_t attn_status_word(uint32_t** p);
+cudaError_t prompt_status_word(uint32_t** p);
 
 template <typename Sym>
-inline int status_take(Sym& word, uint32_t* bits, cudaStream_t st) {
-  const uint32_t zero = 0;
-  cudaError_t e = cudaMemcpyFromSymbolAsync(bits, word, sizeof zero, 0, cudaMemcpyDeviceToHost, st);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-  if (e == cudaSuccess) e = cudaMemcpyToSymbolAsync(word, &zero, sizeof zero, 0, cudaMemcpyHostToDevice, st);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-  if (e != cudaSuccess) return fail(RNB_ERR_CUDA, std::string("rnb_kv_status: ") + cudaGetErrorString(e));
-  return RNB_OK;
+inline cudaError_t status_word(Sym& word, uint32_t** p) {
+  return cudaGetSymbolAddress(reinterpret_cast<void**>(p), word);
 }
 
 // Two fp32 operations in one instruction.

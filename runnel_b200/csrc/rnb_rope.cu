@@ -243,7 +243,7 @@ int launch_rope(const RopeArgs& a, int D, dim3 grid, cudaStream_t st) {
 
 }  // namespace
 
-int rope_status_take(uint32_t* bits, cudaStream_t st) { return status_take(g_rope_status, bits, st); }
+cudaError_t rope_status_word(uint32_t** p) { return status_word(g_rope_status, p); }
 
 }  // namespace rnb
 

@@ -581,6 +581,22 @@ def test_other_streams_and_overlapping_calls():
         assert all(torch.equal(o, want[i]) for o in got[i])
 
 
+def test_status_reads_lose_no_bit_of_another_stream():
+    """A void plan on a side stream, at any moment of a read: its bit is in that read or in a later one."""
+    r, side = random.Random(1), torch.cuda.Stream()
+    t, one, none = _i([[0]]), _i([1]), _i([0])
+    for _ in range(400):
+        done = torch.cuda.Event()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(r.randint(100_000, 500_000))
+            attention.kv_plan(t, none, one, none, none, page_size=16, num_pages=1, max_tokens=1)
+            done.record()
+        seen = 0
+        while not done.query():
+            seen |= attention.status()
+        assert seen | attention.status() == _lib.STATUS_NO_PAGES
+
+
 def test_refusals_on_the_device():
     g = _gen(15)
     kc, vc, table = _cache_of(g, BF16, [20, 20], 2, 64, 16)
