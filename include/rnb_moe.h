@@ -409,10 +409,18 @@ RNB_API int rnb_kv_plan(int B, int table_cols, int page_size, int num_pages, int
 /* Gives the pages of finished requests back: for every b with finished[b] != 0
  * the first ceil(lens[b] / page_size) entries of its table row are appended to
  * free_pages behind *free_count, requests in order, and lens_out[b] = 0 (else
- * lens[b]; lens_out may be lens).  free_count_out as in rnb_kv_plan.  If they
- * do not fit free_capacity, or a length is negative or beyond the table, the
- * call does nothing (lens_out = lens) and sets RNB_STATUS_NO_PAGES.  One CTA:
- * B <= 16384. */
+ * lens[b]; lens_out may be lens).  A negative entry holds no page and is passed
+ * over; so is an id from num_pages on, which sets RNB_STATUS_BAD_INDEX.  Attention
+ * allows any id where it never looks (pages wholly before a window); an entry
+ * whose page was given away there has to be negative by now, or the page is on the
+ * free list twice.  free_count_out as in rnb_kv_plan.  If the pages do not fit
+ * free_capacity, or a length is negative or beyond the table, the call does
+ * nothing (lens_out = lens) and sets RNB_STATUS_NO_PAGES.  One CTA: B <= 16384. */
+RNB_API int rnb_kv_release_bounded(int B, int table_cols, int page_size, int num_pages, const int32_t* table,
+                                   const int32_t* lens, const int32_t* finished, int32_t* free_pages,
+                                   int free_capacity, const int32_t* free_count, int32_t* lens_out,
+                                   int32_t* free_count_out, void* stream);
+/* The same where the caller vouches for the ids: every one from 0 on is a page. */
 RNB_API int rnb_kv_release(int B, int table_cols, int page_size, const int32_t* table, const int32_t* lens,
                            const int32_t* finished, int32_t* free_pages, int free_capacity,
                            const int32_t* free_count, int32_t* lens_out, int32_t* free_count_out, void* stream);

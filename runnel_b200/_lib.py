@@ -128,6 +128,7 @@ SIGNATURES = {
     "rnb_add_rmsnorm": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.c_float, _vp]),
     "rnb_kv_plan": (_i, [_i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "rnb_kv_release": (_i, [_i, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp]),
+    "rnb_kv_release_bounded": (_i, [_i, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp]),
     "rnb_kv_status": (_i, [ctypes.POINTER(ctypes.c_uint32), _vp]),
     "rnb_rope_append": (_i, [ctypes.POINTER(RnbRopeDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _CacheP, _vp, _vp]),
     "rnb_paged_attention_workspace_size": (_i, [ctypes.POINTER(RnbAttnDesc), _CacheP, ctypes.POINTER(_sz)]),

@@ -41,7 +41,7 @@ def _native():
         except ImportError as e:
             raise RuntimeError("runnel_b200/_torch_calls.so is missing or does not load: build it first (python -c "
                                "'import __graft_entry__ as g; g.build()' or make -C runnel_b200/csrc)") from e
-        names = ("rnb_kv_plan", "rnb_kv_release", "rnb_rope_append", "rnb_paged_attention_workspace_size",
+        names = ("rnb_kv_plan", "rnb_kv_release_bounded", "rnb_rope_append", "rnb_paged_attention_workspace_size",
                  "rnb_paged_attention")
         _torch_calls.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names})
         _calls = _torch_calls
@@ -81,11 +81,17 @@ def kv_plan(table: torch.Tensor, ctx_lens: torch.Tensor, new_lens: torch.Tensor,
 
 
 def kv_release(table: torch.Tensor, lens: torch.Tensor, finished: torch.Tensor, free_pages: torch.Tensor,
-               free_count: torch.Tensor, *, page_size: int) -> tuple[torch.Tensor, torch.Tensor]:
+               free_count: torch.Tensor, *, page_size: int, num_pages: int | None = None
+               ) -> tuple[torch.Tensor, torch.Tensor]:
     """Append the pages of requests with ``finished[b] != 0`` (int32) to
     ``free_pages[:free_count]``, in place; returns (lengths with theirs 0, the
-    new count).  Does nothing, with ``STATUS_NO_PAGES``, if they do not fit."""
-    return (_calls or _native()).kv_release(table, lens, finished, free_pages, free_count, page_size)
+    new count).  Does nothing, with ``STATUS_NO_PAGES``, if they do not fit.
+
+    Negative table entries hold no page and are passed over: an entry before a
+    request's window whose page was given away has to be negative by now.  Ids from
+    ``num_pages`` on (None: any is a page) are left out too, with ``STATUS_BAD_INDEX``.
+    """
+    return (_calls or _native()).kv_release(table, lens, finished, free_pages, free_count, page_size, num_pages)
 
 
 def status(device=None) -> int:

@@ -57,7 +57,7 @@ class PagedKVCache:
     def release(self, finished: torch.Tensor) -> None:
         """Requests with ``finished[b] != 0`` (int32) give their pages back and become empty."""
         lens, count = attention.kv_release(self.table, self.lens, finished, self.free_pages, self.free_count,
-                                           page_size=self.page_size)
+                                           page_size=self.page_size, num_pages=self.num_pages)
         self.lens.copy_(lens)
         self.free_count.copy_(count)
 

@@ -170,24 +170,27 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(const PlanArgs a) {
 }
 
 struct ReleaseArgs {
-  int B, W, log2p, free_capacity;
+  int B, W, log2p, num_pages, free_capacity;
   const int32_t *table, *lens, *finished;
   int32_t* free_pages;
   const int32_t* free_count;
   int32_t *lens_out, *free_out;
 };
 
-// One CTA (requests finish one at a time): the pages of all finished requests
-// as one flat range, each found by binary search.
+// One CTA (requests finish one at a time): the table entries of all finished
+// requests as one flat range, each found by binary search, 256 at a time; those
+// that are pages close up in order (a ballot a warp, the warps' counts summed).
 __global__ void __launch_bounds__(kPlanThreads) k_kv_release(const ReleaseArgs a) {
   after_previous();
   extern __shared__ int32_t sh[];
   int32_t* base = sh;        // [B]
   int32_t* none = sh + a.B;  // [B] the second of block_sums' arrays
   __shared__ int64_t wsum[kPlanThreads / 32][2], tot[2];
-  const int tid = threadIdx.x;
+  __shared__ int in_warp[2][kPlanThreads / 32];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int P = 1 << a.log2p;
-  const int fc = *a.free_count;
+  __shared__ int count;  // (one read: barriers below hang on it)
+  if (tid == 0) count = *a.free_count;
   int bad = 0;
   for (int b = tid; b < a.B; b += kPlanThreads) {
     int32_t pages = 0;
@@ -201,14 +204,48 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_release(const ReleaseArgs a
     none[b] = 0;
   }
   bad = __syncthreads_or(bad);
+  const int fc = count;
   block_sums(base, none, a.B, wsum, tot);
-  const bool ok = !bad && fc >= 0 && fc + tot[0] <= a.free_capacity;
-  const int pages = ok ? static_cast<int>(tot[0]) : 0;
-  for (int n = tid; n < pages; n += kPlanThreads) {
+  bool ok = !bad && fc >= 0 && fc <= a.free_capacity && tot[0] < INT32_MAX;
+  const int held = ok ? static_cast<int>(tot[0]) : 0;
+  auto entry = [&](int n) {
     const int b = find_request(base, a.B, n);
-    a.free_pages[fc + n] = a.table[static_cast<int64_t>(b) * a.W + (n - base[b])];
+    return a.table[static_cast<int64_t>(b) * a.W + (n - base[b])];
+  };
+  // entry n's place among the pages of its 256, and how many those are
+  int round = 0;
+  auto place = [&](bool page, int* all) {
+    const uint32_t mask = __ballot_sync(0xffffffffu, page);
+    int* n_in = in_warp[round++ & 1];  // (two in turns: one barrier a round)
+    if (lane == 0) n_in[warp] = __popc(mask);
+    __syncthreads();
+    int at = __popc(mask & ((1u << lane) - 1));
+    *all = 0;
+    for (int w = 0; w < kPlanThreads / 32; ++w) {
+      at += w < warp ? n_in[w] : 0;
+      *all += n_in[w];
+    }
+    return at;
+  };
+  bool strange = false;
+  int pages = 0;
+  // entries that are no pages need no room: where not all entries fit, the pages are counted first
+  for (int pass = held <= a.free_capacity - fc ? 1 : 0; pass < 2 && ok; ++pass) {
+    pages = 0;
+    for (int n0 = 0; n0 < held; n0 += kPlanThreads) {
+      const int id = n0 + tid < held ? entry(n0 + tid) : -1;
+      const bool page = id >= 0 && id < a.num_pages;
+      strange = strange || id >= a.num_pages;
+      int all;
+      const int at = place(page, &all);
+      if (page && pass == 1) a.free_pages[fc + pages + at] = id;
+      pages += all;
+    }
+    ok = pages <= a.free_capacity - fc;
   }
+  if (!ok) pages = 0;
   for (int b = tid; b < a.B; b += kPlanThreads) a.lens_out[b] = ok && a.finished[b] ? 0 : a.lens[b];
+  if (strange) atomicOr(&g_kv_status, RNB_STATUS_BAD_INDEX);
   if (tid == 0) {
     *a.free_out = fc + pages;
     if (!ok) atomicOr(&g_kv_status, RNB_STATUS_NO_PAGES);
@@ -276,12 +313,13 @@ int rnb_kv_plan(int B, int table_cols, int page_size, int num_pages, int max_tok
   return launch("rnb_kv_plan", k_kv_plan, grid, kPlanThreads, smem, static_cast<cudaStream_t>(stream), a);
 }
 
-int rnb_kv_release(int B, int table_cols, int page_size, const int32_t* table, const int32_t* lens,
-                   const int32_t* finished, int32_t* free_pages, int free_capacity, const int32_t* free_count,
-                   int32_t* lens_out, int32_t* free_count_out, void* stream) {
+int rnb_kv_release_bounded(int B, int table_cols, int page_size, int num_pages, const int32_t* table,
+                           const int32_t* lens, const int32_t* finished, int32_t* free_pages, int free_capacity,
+                           const int32_t* free_count, int32_t* lens_out, int32_t* free_count_out, void* stream) {
   using namespace rnb;
   int rc = check_plan(B, table_cols, page_size, "rnb_kv_release");
   if (rc) return rc;
+  if (num_pages <= 0) return fail(RNB_ERR_INVALID, "rnb_kv_release: num_pages must be positive");
   if (free_capacity < 0) return fail(RNB_ERR_INVALID, "rnb_kv_release: free_capacity must be >= 0");
   if ((B && (!table || !lens || !finished || !lens_out)) || !free_count || !free_count_out ||
       (free_capacity && !free_pages))
@@ -291,9 +329,16 @@ int rnb_kv_release(int B, int table_cols, int page_size, const int32_t* table, c
   if ((rc = check_device())) return rc;
   const size_t smem = 8u * static_cast<size_t>(B);
   if ((rc = allow_smem(k_kv_release, smem))) return rc;
-  const ReleaseArgs a{B, table_cols, log2_of(page_size), free_capacity, table, lens, finished, free_pages, free_count,
-                      lens_out, free_count_out};
+  const ReleaseArgs a{B, table_cols, log2_of(page_size), num_pages, free_capacity, table, lens, finished, free_pages,
+                      free_count, lens_out, free_count_out};
   return launch("rnb_kv_release", k_kv_release, 1, kPlanThreads, smem, static_cast<cudaStream_t>(stream), a);
+}
+
+int rnb_kv_release(int B, int table_cols, int page_size, const int32_t* table, const int32_t* lens,
+                   const int32_t* finished, int32_t* free_pages, int free_capacity, const int32_t* free_count,
+                   int32_t* lens_out, int32_t* free_count_out, void* stream) {
+  return rnb_kv_release_bounded(B, table_cols, page_size, INT32_MAX, table, lens, finished, free_pages, free_capacity,
+                                free_count, lens_out, free_count_out, stream);
 }
 
 int rnb_kv_status(uint32_t* status, void* stream) {

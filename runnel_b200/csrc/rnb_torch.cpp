@@ -26,7 +26,7 @@ namespace {
 
 struct Fns {
   decltype(&rnb_kv_plan) kv_plan = nullptr;
-  decltype(&rnb_kv_release) kv_release = nullptr;
+  decltype(&rnb_kv_release_bounded) kv_release = nullptr;
   decltype(&rnb_rope_append) rope_append = nullptr;
   decltype(&rnb_paged_attention_workspace_size) workspace_size = nullptr;
   decltype(&rnb_paged_attention) paged_attention = nullptr;
@@ -34,7 +34,7 @@ struct Fns {
 
 void bind(const std::map<std::string, uintptr_t>& at) {
   fns.kv_plan = reinterpret_cast<decltype(fns.kv_plan)>(at.at("rnb_kv_plan"));
-  fns.kv_release = reinterpret_cast<decltype(fns.kv_release)>(at.at("rnb_kv_release"));
+  fns.kv_release = reinterpret_cast<decltype(fns.kv_release)>(at.at("rnb_kv_release_bounded"));
   fns.rope_append = reinterpret_cast<decltype(fns.rope_append)>(at.at("rnb_rope_append"));
   fns.workspace_size = reinterpret_cast<decltype(fns.workspace_size)>(at.at("rnb_paged_attention_workspace_size"));
   fns.paged_attention = reinterpret_cast<decltype(fns.paged_attention)>(at.at("rnb_paged_attention"));
@@ -181,7 +181,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> kv_plan(const Tensor& table, 
 }
 
 std::tuple<Tensor, Tensor> kv_release(const Tensor& table, const Tensor& lens, const Tensor& finished,
-                                      const Tensor& free_pages, const Tensor& free_count, int64_t page_size) {
+                                      const Tensor& free_pages, const Tensor& free_count, int64_t page_size,
+                                      std::optional<int64_t> num_pages) {
   const at::Device dev = cuda_device(table, "table");
   if (table.dim() != 2) refuse("table must be [requests, columns]");
   const int64_t B = table.size(0), cols = table.size(1);
@@ -193,7 +194,8 @@ std::tuple<Tensor, Tensor> kv_release(const Tensor& table, const Tensor& lens, c
   const c10::cuda::CUDAGuard guard(dev);
   Tensor out = empty({B}, at::kInt, dev), left = empty({1}, at::kInt, dev);
   check("rnb_kv_release",
-        fns.kv_release(c_int(B, "requests"), c_int(cols, "columns"), c_int(page_size, "page_size"), tp, lp, np, fp,
+        fns.kv_release(c_int(B, "requests"), c_int(cols, "columns"), c_int(page_size, "page_size"),
+                       c_int(num_pages.value_or(INT32_MAX), "num_pages"), tp, lp, np, fp,
                        c_int(free_pages.numel(), "free_pages"), fc, static_cast<int32_t*>(out.data_ptr()),
                        static_cast<int32_t*>(left.data_ptr()), stream_of(dev)));
   return {out, left};

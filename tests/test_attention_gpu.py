@@ -151,6 +151,43 @@ def test_release_returns_pages_in_order():
     assert attention.status() == _lib.STATUS_NO_PAGES
 
 
+def test_release_passes_over_entries_without_a_page():
+    """Entries given away before a window, and ids beyond the cache, do not come back as free pages."""
+    table, lens, fin = _i([[-1, -1, 3], [6, 7, 8], [4, 12, 5]]), _i([48, 33, 40]), _i([1, 0, 1])
+    free = _i([9, -1, -1, -1, -1])
+    out, n = attention.kv_release(table, lens, fin, free, _i([1]), page_size=16, num_pages=12)
+    assert free.tolist() == [9, 3, 4, 5, -1] and n.item() == 4 and out.tolist() == [0, 33, 0]
+    assert attention.status() == _lib.STATUS_BAD_INDEX
+    p = attention.kv_plan(table, out, _i([20, 0, 17]), free, n, page_size=16, num_pages=12, max_tokens=37)
+    assert table.tolist() == [[5, 4, 3], [6, 7, 8], [3, 9, 5]] and p.free_count.item() == 0
+    assert attention.status() == 0
+    # without num_pages every id from 0 on is a page
+    free = _i([9, -1, -1, -1, -1])
+    attention.kv_release(_i([[-1, 12, -2 ** 31]]), _i([48]), _i([1]), free, _i([1]), page_size=16)
+    assert free.tolist() == [9, 12, -1, -1, -1] and attention.status() == 0
+
+
+@pytest.mark.parametrize("B,W", [(1, 1), (1, 300), (7, 100), (300, 9), (2, 5000)])
+@pytest.mark.parametrize("gone", [0.0, 0.3, 1.0])
+def test_release_of_any_length(B, W, gone):
+    """The free list is just long enough, and one too short."""
+    r = random.Random(B * W)
+    lens = [r.choice([0, 1, 16 * W, r.randint(0, 16 * W)]) for _ in range(B)]
+    lens[0], fin = 16 * W, [1] + [int(r.random() < 0.7) for _ in range(B - 1)]
+    table = [[r.choice([-1, -9]) if r.random() < gone else b * W + j for j in range(W)] for b in range(B)]
+    back = [e for b in range(B) if fin[b] for e in table[b][:-(-lens[b] // 16)] if e >= 0]
+    t, ln, fn = _i(table).view(B, W), _i(lens), _i(fin)
+    free = torch.full((2 + len(back),), -7, dtype=torch.int32, device=DEV)
+    out, n = attention.kv_release(t, ln, fn, free, _i([2]), page_size=16, num_pages=B * W)
+    assert free.tolist() == [-7, -7] + back and n.item() == 2 + len(back)
+    assert out.tolist() == [0 if f else x for x, f in zip(lens, fin)] and attention.status() == 0
+    if back:
+        free = torch.full((1 + len(back),), -7, dtype=torch.int32, device=DEV)
+        out, n = attention.kv_release(t, ln, fn, free, _i([2]), page_size=16, num_pages=B * W)
+        assert (free == -7).all() and n.item() == 2 and torch.equal(out, ln)
+        assert attention.status() == _lib.STATUS_NO_PAGES
+
+
 # ------------------------------------------------------------------ rotary
 
 def _sections(n, axes):

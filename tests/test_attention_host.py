@@ -48,6 +48,14 @@ def test_release_refuses(kw, msg):
     assert rc == -1 and msg in _err()
 
 
+def test_bounded_release_refuses():
+    def call(cols=8, pages=32, fin=F + 128):
+        return _lib.load().rnb_kv_release_bounded(4, cols, 16, pages, F, F + 64, fin, F + 192, 8, F + 256, F + 64, F + 320,
+                                                  None)
+    for kw, msg in ((dict(pages=0), "num_pages"), (dict(cols=0), "table_cols"), (dict(fin=None), "non-NULL")):
+        assert call(**kw) == -1 and msg in _err()
+
+
 def _kv(**kw):
     c = _lib.RnbKvCache(dtype=0, num_pages=16, page_size=16, n_kv_heads=2, head_dim=128, k=F, v=F,
                         k_page_stride=2 * 16 * 128, k_head_stride=16 * 128, v_page_stride=2 * 16 * 128,
