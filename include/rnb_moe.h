@@ -399,8 +399,10 @@ typedef struct rnb_kv_cache {
  * All or nothing: if the pages, the table's columns, max_tokens or 31 bits do
  * not suffice, or a length is negative, nothing is taken, seq_lens = ctx_lens,
  * cu_q = 0, every slot is -1 and RNB_STATUS_NO_PAGES is set, so the step's
- * later calls do nothing.  A call with the same inputs gives the same outputs
- * again.  B <= 16384.  A page id outside [0, num_pages) gives slot -1 and
+ * later calls do nothing.  So it is where an id that would be taken from the free
+ * list is outside [0, num_pages), with RNB_STATUS_BAD_INDEX too.  A call with the
+ * same inputs gives the same outputs again.  B <= 16384.  A row in a page that the
+ * table held already and whose id is outside [0, num_pages) gets slot -1, with
  * RNB_STATUS_BAD_INDEX. */
 RNB_API int rnb_kv_plan(int B, int table_cols, int page_size, int num_pages, int max_tokens, int32_t* table,
                         const int32_t* ctx_lens, const int32_t* new_lens, const int32_t* free_pages,

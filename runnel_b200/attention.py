@@ -74,7 +74,8 @@ def kv_plan(table: torch.Tensor, ctx_lens: torch.Tensor, new_lens: torch.Tensor,
     All or nothing: where pages, table columns or ``max_tokens`` do not
     suffice, or a length is negative, the plan is void (``cu_q`` 0, slots -1,
     ``seq_lens`` = ``ctx_lens``, nothing taken) and :func:`status` has
-    ``STATUS_NO_PAGES``.
+    ``STATUS_NO_PAGES``; so it is where the free list's ids that it would take are
+    not all in ``[0, num_pages)``, with ``STATUS_BAD_INDEX`` too.
     """
     return KVPlan(*(_calls or _native()).kv_plan(table, ctx_lens, new_lens, free_pages, free_count, page_size, num_pages,
                                                  max_tokens))

