@@ -102,6 +102,22 @@ def test_plan_ragged(B, P, most_ctx, most_new):
     _check_plan(ctx, new, P, W, sum(new) + 5, seed=B)
 
 
+@pytest.mark.parametrize("B", [6000, 6016, 6017, 6126, 6127, 6144, 6145, 16384])
+def test_plan_and_release_of_any_batch(B):
+    """Batches around the border of the shared memory that a kernel has unasked."""
+    r = random.Random(B)
+    ctx, new = [r.randint(0, 40) for _ in range(B)], [r.randint(0, 2) for _ in range(B)]
+    _check_plan(ctx, new, 16, 3, sum(new) + 1, seed=B)
+    lens, fin = [r.randint(0, 32) for _ in range(B)], [int(r.random() < 0.3) for _ in range(B)]
+    table = torch.arange(2 * B, dtype=torch.int32, device=DEV).view(B, 2)
+    free = torch.full((2 * B,), -5, dtype=torch.int32, device=DEV)
+    out, n = attention.kv_release(table, _i(lens), _i(fin), free, _i([0]), page_size=16)
+    want = [2 * b + j for b in range(B) if fin[b] for j in range(-(-lens[b] // 16))]
+    assert free.tolist() == want + [-5] * (2 * B - len(want)) and n.item() == len(want)
+    assert out.tolist() == [0 if f else x for x, f in zip(lens, fin)]
+    assert attention.status() == 0
+
+
 @pytest.mark.parametrize("ctx,new,W,cap,short", [
     ([10, 0], [10, 40], 4, 50, 1),  # a page too few
     ([10, 0], [10, 40], 4, 49, 0),  # a token row too few
