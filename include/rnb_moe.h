@@ -489,9 +489,9 @@ RNB_API int rnb_rope_append(const rnb_rope_desc* d, const void* q, const void* k
  * must be finite where any of the request's rows sees them: what lies before the
  * window of its first row may have any bits, and pages wholly before it any id.
  * Any number of rows per request; requests in any mix.  out may be q where q is
- * packed; otherwise it shares no memory with q or gate.  max_q (0: unknown)
- * bounds the rows of a request and only picks the kernels.  The workspace needs
- * no initial state; calls that may overlap need one each.  Results do not depend
+ * packed; otherwise an out that shares memory with q or gate is refused.  max_q
+ * (0: unknown) bounds the rows of a request and only picks the kernels.  The
+ * workspace needs no initial state; calls that may overlap need one each.  Results do not depend
  * on timing: equal inputs give equal bits.  A device wait inside the many-row
  * kernel that gives up after a second sets RNB_STATUS_TIMEOUT: results are void
  * then, and until the status is read many-row requests are left out. */

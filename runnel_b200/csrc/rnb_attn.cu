@@ -793,6 +793,16 @@ int rnb_paged_attention(const rnb_attn_desc* d, const rnb_kv_cache* cache, const
     return fail(RNB_ERR_INVALID, "rnb_paged_attention: q, out, table and seq_lens must be non-NULL");
   if (!aligned16(q) || !aligned16(gate) || !aligned16(out) || !aligned16(ws))
     return fail(RNB_ERR_ALIGN, "rnb_paged_attention: q, gate, out and the workspace must be 16-byte aligned");
+  // CTAs write rows of out while others still read theirs of q and gate
+  const int64_t D = cache->head_dim;
+  const bool in_place = out == q && (d->T == 1 || d->q_token_stride == D * d->n_q_heads) &&
+                        (d->n_q_heads == 1 || d->q_head_stride == D);
+  if (!in_place && shares_memory(out, d->T, d->n_q_heads, D, q, d->q_token_stride, d->q_head_stride, d->n_q_heads))
+    return fail(RNB_ERR_INVALID,
+                "rnb_paged_attention: out may be q where q is packed [T][n_q_heads][head_dim]; otherwise they must not "
+                "share memory");
+  if (shares_memory(out, d->T, d->n_q_heads, D, gate, d->gate_token_stride, d->gate_head_stride, d->n_q_heads))
+    return fail(RNB_ERR_INVALID, "rnb_paged_attention: out and gate must not share memory");
   if ((rc = check_device())) return rc;
   const Plan p = plan_of(d, cache, dev_info().sms, cu_q != nullptr);
   if (!ws || ws_bytes < p.bytes)

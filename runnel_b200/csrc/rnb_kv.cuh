@@ -39,6 +39,25 @@ inline int check_cache(const rnb_kv_cache* c, const char* fn) {
   return RNB_OK;
 }
 
+// Whether a packed output [T][H][D] of 16-bit elements shares memory with rows
+// (T tokens, `heads` heads of D elements, strides >= 0 in elements).  Row by row
+// where the ranges as a whole overlap: an output may lie in the gaps.
+inline bool shares_memory(const void* out, int64_t T, int64_t H, int64_t D, const void* rows, int64_t token_stride,
+                          int64_t head_stride, int64_t heads) {
+  const uintptr_t o0 = reinterpret_cast<uintptr_t>(out), o1 = o0 + 2 * T * H * D;
+  auto meets = [&](int64_t from, int64_t n) {  // n elements from `from` on
+    const uintptr_t r0 = reinterpret_cast<uintptr_t>(rows) + 2 * from;
+    return r0 < o1 && r0 + 2 * n > o0;
+  };
+  const int64_t token = (heads - 1) * head_stride + D;
+  if (!rows || T == 0 || heads == 0 || !meets(0, (T - 1) * token_stride + token)) return false;
+  for (int64_t t = 0; t < T; ++t)
+    if (meets(t * token_stride, token))
+      for (int64_t h = 0; h < heads; ++h)
+        if (meets(t * token_stride + h * head_stride, D)) return true;
+  return false;
+}
+
 // A launch whose grid may come up while the kernel before it in the stream ends
 // (programmatic dependent launch; 1 us less between two small kernels).  Every
 // kernel launched so waits for that one (griddep_wait) before anything else, its

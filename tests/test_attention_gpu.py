@@ -583,6 +583,25 @@ def test_strided_queries_gates_and_caches():
                                                      gate=gate), a)
 
 
+def test_outputs_over_strided_queries_are_refused():
+    """The query part of a joint projection is not packed: out may not lie there."""
+    g = _gen(33)
+    kc, vc, table = _cache_of(g, BF16, [50, 60, 70], 2, 64, 16)
+    buf = _rand(g, BF16, 3 * 8 * 64 * 3)
+    joint = buf[:3 * 8 * 128].view(3, 8, 128)
+    was, sl = buf.clone(), _i([50, 60, 70])
+    out = buf[:3 * 8 * 64].view(3, 8, 64)
+    with pytest.raises(_lib.RnbError, match="packed"):
+        attention.paged_attention(joint[..., :64], kc, vc, table, sl, out=out)
+    with pytest.raises(_lib.RnbError, match="gate"):
+        attention.paged_attention(joint[..., :64].contiguous(), kc, vc, table, sl, gate=joint[..., 64:], out=out)
+    assert torch.equal(buf, was)
+    behind = buf[3 * 8 * 128:].view(3, 8, 64)
+    want = attention.paged_attention(joint[..., :64], kc, vc, table, sl, gate=joint[..., 64:])
+    assert torch.equal(attention.paged_attention(joint[..., :64], kc, vc, table, sl, gate=joint[..., 64:], out=behind), want)
+    assert attention.status() == 0
+
+
 def test_rows_behind_the_last_request_stay():
     g = _gen(11)
     lens, rows = [100, 200], [3, 80]

@@ -100,6 +100,29 @@ def test_attention_refuses(kw, code, msg):
     assert _attn(**kw) == code and msg in _err()
 
 
+@pytest.mark.parametrize("kw,msg", [
+    (dict(q_token_stride=2048, q_head_stride=256), "packed"),  # out at the head of interleaved queries
+    (dict(out=F + 4 * 2048 - 16), "packed"), (dict(out=F + 64), "packed"), (dict(q=F + 4 * 2048 - 16), "packed"),
+    (dict(gate=F, q=F + 8192, gate_token_stride=1024, gate_head_stride=128), "gate"),
+    (dict(gate=F + 8192 - 256, q=F + 32768, gate_token_stride=2048, gate_head_stride=128), "gate"),
+])
+def test_attention_refuses_outputs_over_its_inputs(kw, msg):
+    assert _attn(**kw) == -1 and msg in _err()
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="a CUDA device is present")
+@pytest.mark.parametrize("kw", [
+    dict(), dict(q=F + 8192), dict(out=F + 8192), dict(q_token_stride=2048, out=F + 16384),
+    dict(T=1, B=1, q_token_stride=8),  # a stride over one token is never used
+    dict(gate=F + 8192, gate_token_stride=1024, gate_head_stride=128),
+    dict(q=F + 8192, q_token_stride=8192, T=1, B=1),
+    dict(T=2, B=2, q=F + 1024, out=F + 4096, n_q_heads=4, q_token_stride=8192, q_head_stride=128),  # between two tokens
+])
+def test_attention_takes_outputs_beside_its_inputs(kw):
+    """(what is refused here is the missing device)"""
+    assert _attn(**kw) == -5
+
+
 def test_attention_of_nothing_is_ok():
     assert _attn(B=0, T=0, q=None, out=None, table=None, seq=None, ws=None, nbytes=0) == 0
 
