@@ -445,8 +445,9 @@ RNB_API int rnb_kv_status(uint32_t* status, void* stream);
  * section after the other (interleaved 0), or in turns (interleaved 1: axis
  * a >= 1 has i = a, a + n_axes, ..., sections[a] of them; axis 0 the rest).
  * Queries go to q_out [T][n_q_heads][head_dim] (may be q itself if q is
- * packed like that); rotated keys and values (as they are) go to the cache
- * row of slots[t].  A row with slots[t] < 0 is left alone altogether; with a
+ * packed like that, and is refused where it shares memory with q, k or v
+ * otherwise); rotated keys and values (as they are) go to the cache row of
+ * slots[t].  A row with slots[t] < 0 is left alone altogether; with a
  * slot beyond the cache only its query is written, and RNB_STATUS_BAD_INDEX
  * is set.  Two rows of one call with the same slot leave either's values.
  * cache, k, v and slots may be NULL together: then only the queries are

@@ -125,7 +125,8 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     frequencies each axis (for images: time, height, width) turns, one section
     after the other, or in turns with ``interleaved``.  Rows with slot -1 are
     left alone, in ``out`` too; the other slots are distinct (of two tokens in one,
-    either may stay).  ``out`` may be ``q`` if that is contiguous.
+    either may stay).  ``out`` may be ``q`` if that is contiguous, but not share memory
+    with ``q``, ``k`` or ``v`` otherwise.
     """
     if k_cache is None or slots is None:
         raise ValueError("rope_append needs a cache and slots; rope() turns queries without them")

@@ -274,6 +274,12 @@ extern "C" int rnb_rope_append(const rnb_rope_desc* d, const void* q, const void
   if (q == q_out && (d->q_head_stride != D || d->q_token_stride != D * d->n_q_heads))
     return fail(RNB_ERR_INVALID, "rnb_rope_append: q_out may be q only if q is packed [T][n_q_heads][head_dim]");
   if ((rc = check_device())) return rc;
+  // groups write rows of q_out while others still read theirs
+  if ((q != q_out &&
+       shares_memory(q_out, d->T, d->n_q_heads, D, q, d->q_token_stride, d->q_head_stride, d->n_q_heads)) ||
+      shares_memory(q_out, d->T, d->n_q_heads, D, k, d->k_token_stride, d->k_head_stride, d->n_kv_heads) ||
+      shares_memory(q_out, d->T, d->n_q_heads, D, v, d->v_token_stride, d->v_head_stride, d->n_kv_heads))
+    return fail(RNB_ERR_INVALID, "rnb_rope_append: q_out must not share memory with q (unless it is q), k or v");
 
   RopeArgs a{};
   a.q = q, a.k = k, a.v = v, a.qw = q_norm_w, a.kw = k_norm_w;

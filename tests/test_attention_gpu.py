@@ -287,6 +287,35 @@ def test_rope_of_text_positions_and_in_place():
     assert attention.rope(x[:0], pos[:0], inv).shape == (0, 6, 128)
 
 
+def test_rope_outputs_over_inputs_are_refused():
+    g = _gen(34)
+    T, D = 4, 64
+    buf = _rand(g, BF16, 2 * T * 16 * D)
+    joint = buf[:T * 12 * D].view(T, 12, D)  # eight query heads, two key, two value heads
+    q, k, v = joint.split([8, 2, 2], 1)
+    kc, vc = _rand(g, BF16, 2, 2, 16, D), _rand(g, BF16, 2, 2, 16, D)
+    inv, pos, slots = torch.rand(32, generator=g, device=DEV), _i([0, 1, 2, 3]), _i([3, 20, 1, 0])
+    n, packed = T * 8 * D, _rand(g, BF16, T, 8, D)
+    was = buf.clone(), kc.clone(), vc.clone()
+    apart = [x.contiguous() for x in (q, k, v)]
+    over = lambda at: buf[at:at + n].view(T, 8, D)  # noqa: E731
+    for qq, kk, vv, out in ((q, apart[1], apart[2], over(0)), (packed, k, apart[2], over(8 * D + 64)),
+                            (packed, apart[1], v, over(T * 12 * D - 64)), (buf[64:64 + n].view(T, 8, D), *apart[1:], over(0))):
+        with pytest.raises(_lib.RnbError, match="share memory|packed"):
+            attention.rope_append(qq, kk, vv, pos, inv, slots, kc, vc, out=out)
+    with pytest.raises(_lib.RnbError, match="share memory|packed"):
+        attention.rope(q, pos, inv, out=over(0))
+    assert all(torch.equal(a, b) for a, b in zip((buf, kc, vc), was))
+    want = attention.rope_append(*apart, pos, inv, slots, kc, vc)
+    assert torch.equal(attention.rope_append(q, k, v, pos, inv, slots, kc, vc, out=over(T * 12 * D)), want)
+    # two tokens of heads 0-7, and their outputs between the joint rows of a wider buffer
+    wide = _rand(g, BF16, 2, 3 * 8 * D)
+    qw = wide[:, :8 * D].view(2, 8, D)
+    want = attention.rope(qw.contiguous(), pos[:2], inv)
+    out = wide.view(-1)[8 * D:24 * D].view(2, 8, D)
+    assert torch.equal(attention.rope(qw, pos[:2], inv, out=out), want)
+
+
 def test_rope_slot_beyond_the_cache_and_negative_positions():
     g = _gen(4)
     q, k, v = (_rand(g, FP16, 3, 2, 64) for _ in range(3))
