@@ -484,7 +484,8 @@ RNB_API int rnb_rope_append(const rnb_rope_desc* d, const void* q, const void* k
  * times sigmoid(gate[t][h]) elementwise when gate is given, rounded once;
  * lse[t][h] (optional, fp32) = log sum_j exp(scale * q . k_j).  A row that
  * sees nothing gives zeros and -inf.  Rows behind cu_q[B] are left as they
- * were.  Softmax statistics and sums are fp32; probabilities are rounded to
+ * were.  Bounds in cu_q that descend or leave [0, T] are cut to what they can mean
+ * inside the tensors, and set RNB_STATUS_BAD_INDEX, as lengths outside the table do.  Softmax statistics and sums are fp32; probabilities are rounded to
  * the cache's type for the product with V.  What lies in the cache behind a
  * request's length never counts, whatever its bits; within the length values
  * must be finite where any of the request's rows sees them: what lies before the

@@ -160,7 +160,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_attn_few(const AttnArgs a) {
     const int lo = min(tid * per, a.B), hi = min(lo + per, a.B);
     auto units = [&](int b) {
       read_request(a, b, c0, c1, len);
-      if (blockIdx.x == 0 && (len < 0 || len > a.max_kv)) atomicOr(&g_attn_status, RNB_STATUS_BAD_INDEX);
+      if (blockIdx.x == 0 && (len < 0 || len > a.max_kv || c0 < 0 || c1 < c0 || c1 > a.T))
+        atomicOr(&g_attn_status, RNB_STATUS_BAD_INDEX);
       const Request r = request_of<R>(a, c0, c1, len);
       return static_cast<int64_t>(r.ntile) * (r.nblk + kTile) * a.Hkv;
     };

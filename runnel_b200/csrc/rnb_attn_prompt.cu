@@ -253,6 +253,9 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
   {
     if (tid == 0) {
       found[0] = -1;
+      // (of several requests the few-row kernel tells)
+      if (a.B == 1 && blockIdx.x == 0 && (a.cu[0] < 0 || a.cu[1] < a.cu[0] || a.cu[1] > a.T))
+        atomicOr(&g_prompt_status, RNB_STATUS_BAD_INDEX);
       // after a wait that gave up, until the status is read: a grid of CTAs that
       // each wait their second would hold the device for minutes
       gave_up = *const_cast<volatile uint32_t*>(&g_prompt_status) & RNB_STATUS_TIMEOUT;
@@ -292,7 +295,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
       int64_t rem = want - base;
       int b = lo;
       int n = per == 1 ? static_cast<int>(sum) : tiles(b);
-      while (rem >= n) {
+      while (rem >= n && b + 1 < hi) {  // (the second: row bounds that change under way must not lead out)
         rem -= n;
         n = tiles(++b);
       }

@@ -700,6 +700,21 @@ def test_other_streams_and_overlapping_calls():
         assert all(torch.equal(o, want[i]) for o in got[i])
 
 
+@pytest.mark.parametrize("max_q", [None, 3])
+@pytest.mark.parametrize("D,Hq,Hkv", [(64, 4, 2), (256, 16, 2), (128, 32, 1)])
+def test_bad_row_bounds_are_told(D, Hq, Hkv, max_q):
+    """Row bounds outside the tensors or descending set a bit, whichever kernel has the requests; others do not."""
+    g, lens = _gen(13), [50, 60]
+    kc, vc, table = _cache_of(g, BF16, lens, Hkv, D, 16)
+    q = _rand(g, BF16, 6, Hq, D)
+    for cu in ([-1, 2, 6], [0, 2, 7], [0, 4, 3], [0, 7], [-2, 6], [3, 1], [7, 7]):
+        attention.paged_attention(q, kc, vc, table[:len(cu) - 1], _i(lens[:len(cu) - 1]), cu_q=_i(cu), max_q=max_q)
+        assert attention.status() == _lib.STATUS_BAD_INDEX, cu
+    for cu in ([0, 2, 6], [1, 2, 4], [3, 3, 3], [0, 6], [6, 6], [2, 3]):
+        attention.paged_attention(q, kc, vc, table[:len(cu) - 1], _i(lens[:len(cu) - 1]), cu_q=_i(cu), max_q=max_q)
+        assert attention.status() == 0, cu
+
+
 def test_status_reads_lose_no_bit_of_another_stream():
     """A void plan on a side stream, at any moment of a read: its bit is in that read or in a later one."""
     r, side = random.Random(1), torch.cuda.Stream()
