@@ -93,7 +93,7 @@ class GatedAttention(torch.nn.Module):
         super().__init__()
         if len({(p.bits, p.group_size, p.mode) for p in (q_proj, k_proj, v_proj)}) != 1:
             raise ValueError("q, k and v projections must share one quantization format")
-        for p in (q_proj, o_proj):
+        for p in (q_proj, k_proj, v_proj, o_proj):
             if p.group_size != 64 or p.mode != "affine" or p.get("biases") is None or "bias" in p:
                 raise ValueError("projections must be affine-quantized in groups of 64, without module biases")
         self.head_dim, self.rotary, self.gated, self.eps = head_dim, rotary, gated, eps

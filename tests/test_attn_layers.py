@@ -56,6 +56,30 @@ def test_attention_layer_on_cpu_refuses_mixed_formats(tmp_path):
         attn_layers.GatedAttention(bad, kv, kv, layer.o_proj, layer.q_norm, layer.k_norm, 64, layer.rotary)
 
 
+@pytest.mark.parametrize("proj", ["q_proj", "k_proj", "v_proj", "o_proj"])
+def test_attention_layer_refuses_what_its_products_would_leave_out(proj):
+    """Module biases and projections without affine biases, in each of the four."""
+    rng = np.random.default_rng(4)
+
+    def linear(rows, K, affine=True):
+        w, s, b = (torch.from_numpy(a.view(np.int32 if a.dtype == np.uint32 else np.int16))
+                   for a in _linear_arrays(rng, rows, K, 4))
+        return QuantizedLinear(w.view(torch.uint32), s.view(torch.bfloat16), b.view(torch.bfloat16) if affine else None)
+
+    def layer(**other):
+        lin = dict(q_proj=linear(1024, 512), k_proj=linear(128, 512), v_proj=linear(128, 512), o_proj=linear(512, 512))
+        lin.update(other)
+        return attn_layers.GatedAttention(**lin, q_norm=None, k_norm=None, head_dim=64, rotary=attn_layers.RotarySpec(32))
+
+    assert layer().n_kv_heads == 2
+    rows = {"q_proj": 1024, "o_proj": 512}.get(proj, 128)
+    biased = linear(rows, 512)
+    biased.register_buffer("bias", torch.zeros(rows))
+    for bad in (biased, linear(rows, 512, affine=False)):
+        with pytest.raises(ValueError, match="affine|format"):
+            layer(**{proj: bad})
+
+
 def test_stack_checks_its_attention_layers():
     with pytest.raises(ValueError, match="attn_norm_w"):
         stack.LayerStack([object()], [object()], attn=[object()])
