@@ -363,19 +363,28 @@ def load_block(store: TensorStore, layer: int, device="cuda", E_range: tuple[int
 def load_attention_arrays(store: TensorStore, layer: int) -> dict:
     """numpy arrays of a full-attention layer's ``self_attn`` (weight, scales, biases of
     each projection, the head norms) and its ``input_layernorm``, with the sizes
-    they imply: head_dim, n_heads, n_kv_heads, gated, and bits per projection."""
+    they imply: head_dim, n_heads, n_kv_heads, gated, and bits per projection.
+    Codes have to be stored as U32, everything else as BF16."""
     p = f"language_model.model.layers.{layer}.self_attn"
     if f"{p}.q_proj.weight" not in store:
         raise ValueError(f"layer {layer} has no full attention")
+
+    def read(name: str, dtype: str) -> np.ndarray:
+        if name in store and store.entries[name][3] != dtype:
+            raise ValueError(f"{name} is {store.entries[name][3]}, not {dtype}")
+        return store.read(name)[0]
+
     out = {"bits": {}}
-    out["q_norm"] = store.read(f"{p}.q_norm.weight")[0]
-    out["k_norm"] = store.read(f"{p}.k_norm.weight")[0]
+    out["q_norm"] = read(f"{p}.q_norm.weight", "BF16")
+    out["k_norm"] = read(f"{p}.k_norm.weight", "BF16")
     D = out["q_norm"].shape[0]
-    norm = f"language_model.model.layers.{layer}.input_layernorm.weight"
-    out["norm_w"] = store.read(norm)[0]
+    out["norm_w"] = read(f"language_model.model.layers.{layer}.input_layernorm.weight", "BF16")
     H = out["norm_w"].shape[0]
     for proj in ("q", "k", "v", "o"):
-        w, s, b = (store.read(f"{p}.{proj}_proj.{n}")[0] for n in ("weight", "scales", "biases"))
+        base = f"{p}.{proj}_proj"
+        if f"{base}.bias" in store:
+            raise ValueError(f"{base}.bias: module biases are not expected")
+        w, s, b = read(f"{base}.weight", "U32"), read(f"{base}.scales", "BF16"), read(f"{base}.biases", "BF16")
         K = s.shape[-1] * 64
         bits = _bits_of(w.shape[-1], K)
         if bits == 0 or (proj != "o" and K != H) or (proj == "o" and w.shape[0] != H):

@@ -43,6 +43,24 @@ def test_checkpoint_attention_arrays(tmp_path, gated):
         checkpoint.load_attention_arrays(st, 0)
 
 
+def test_checkpoint_attention_refuses_other_types_and_biases(tmp_path):
+    """Scales, biases and norms are taken as bf16 bits and codes as 32-bit words; a projection's own bias has no place."""
+    p = "language_model.model.layers.3"
+    odd = {f"{p}.input_layernorm.weight": "F16", f"{p}.self_attn.q_norm.weight": "F16",
+           f"{p}.self_attn.k_norm.weight": "F32", f"{p}.self_attn.v_proj.scales": "F16",
+           f"{p}.self_attn.o_proj.biases": "F16", f"{p}.self_attn.k_proj.weight": "I32",
+           f"{p}.self_attn.q_proj.bias": "BF16", f"{p}.self_attn.o_proj.bias": "BF16"}
+    st = _write(tmp_path, np.random.default_rng(5), 512, 8, 2, 64)
+    good = {n: (st.read(n)[0], e[3]) for n, e in st.entries.items()}
+    for name, dtype in odd.items():
+        arr = good[name][0] if name in good else np.zeros(512, np.uint16)
+        checkpoint.write_safetensors(str(tmp_path / "model.safetensors"), {**good, name: (arr, dtype)})
+        with pytest.raises(ValueError, match=name):
+            checkpoint.load_attention_arrays(checkpoint.TensorStore(str(tmp_path)), 3)
+    checkpoint.write_safetensors(str(tmp_path / "model.safetensors"), good)
+    assert checkpoint.load_attention_arrays(checkpoint.TensorStore(str(tmp_path)), 3)["n_heads"] == 8
+
+
 def test_attention_layer_on_cpu_refuses_mixed_formats(tmp_path):
     st = _write(tmp_path, np.random.default_rng(1), 512, 8, 2, 64, bits=(4, 8, 4, 8))
     with pytest.raises(ValueError, match="one quantization format"):
