@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import os
 import subprocess
+import sys
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -169,7 +170,7 @@ class RnbError(RuntimeError):
 
 def build() -> str:
     """Compile the CUDA library in-tree with nvcc (sm_100a)."""
-    subprocess.run(["make", "-s", "-C", os.path.join(_HERE, "csrc")], check=True)
+    subprocess.run(["make", "-s", "-C", os.path.join(_HERE, "csrc"), f"PYTHON={sys.executable}"], check=True)
     return LIB_PATH
 
 

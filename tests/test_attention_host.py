@@ -2,6 +2,9 @@
 alignment and aliasing are checked on the host before any device work, so the
 pointers here are never used."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -201,3 +204,11 @@ def test_python_refuses_cpu_tensors():
         attention.rope_append(q, q, q, i, torch.zeros(16), None, kc, kc)
     with pytest.raises(ValueError, match="CUDA"):
         attention.status("cpu")
+
+
+def test_extension_module_is_rebuilt_for_another_torch():
+    """It holds torch's inline code: a torch installed later makes it out of date."""
+    here = os.path.dirname(os.path.abspath(_lib.__file__))
+    version = os.path.join(os.path.dirname(torch.__file__), "version.py")
+    cmd = ["make", "-n", "-C", os.path.join(here, "csrc"), f"PYTHON={sys.executable}", os.path.join(here, "_torch_calls.so")]
+    assert "rnb_torch.cpp" in subprocess.run(cmd + ["-W", version], capture_output=True, text=True, check=True).stdout
