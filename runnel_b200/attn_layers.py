@@ -42,20 +42,29 @@ class PagedKVCache:
         # taken from the end: page 0 first
         self.free_pages = torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=device)
         self.free_count = torch.full((1,), num_pages, dtype=torch.int32, device=device)
+        self._stale = False  # a release came after the last plan
+        self._captured = False  # a plan is part of a graph, whose replays are not seen here
 
     def plan(self, new_lens: torch.Tensor, max_tokens: int) -> attention.KVPlan:
         """Pages, slots and positions for ``new_lens`` ``[max_requests]`` more tokens;
         nothing is taken over before :meth:`commit`."""
+        self._stale = False
+        self._captured = self._captured or (self.lens.is_cuda and torch.cuda.is_current_stream_capturing())
         return attention.kv_plan(self.table, self.lens, new_lens, self.free_pages, self.free_count,
                                  page_size=self.page_size, num_pages=self.num_pages, max_tokens=max_tokens)
 
     def commit(self, plan: attention.KVPlan) -> None:
-        """The step's tokens are cached now (in place, so captured steps keep their addresses)."""
+        """The step's tokens are cached now (in place, so captured steps keep their addresses).
+        A plan from before a :meth:`release` is refused: its lengths and free count would undo it."""
+        if self._stale and not self._captured:
+            raise RuntimeError("pages were released after this plan: plan again")
         self.lens.copy_(plan.seq_lens)
         self.free_count.copy_(plan.free_count)
 
     def release(self, finished: torch.Tensor) -> None:
-        """Requests with ``finished[b] != 0`` (int32) give their pages back and become empty."""
+        """Requests with ``finished[b] != 0`` (int32) give their pages back and become empty;
+        between a step's :meth:`commit` and the next :meth:`plan`, or instead of a commit."""
+        self._stale = True
         lens, count = attention.kv_release(self.table, self.lens, finished, self.free_pages, self.free_count,
                                            page_size=self.page_size, num_pages=self.num_pages)
         self.lens.copy_(lens)

@@ -98,6 +98,23 @@ def test_attention_layer_refuses_what_its_products_would_leave_out(proj):
             layer(**{proj: bad})
 
 
+def test_a_release_makes_plans_stale(monkeypatch):
+    """(the calls are stood in for: what is tested is the order)"""
+    cache = _cache(1, 2, 64, 3, device="cpu")
+    plan = attention.KVPlan(cache.lens + 1, None, None, None, cache.free_count - 1)
+    monkeypatch.setattr(attention, "kv_plan", lambda *a, **k: plan)
+    monkeypatch.setattr(attention, "kv_release", lambda *a, **k: (cache.lens * 0, cache.free_count + 3))
+    cache.commit(cache.plan(None, 3))
+    assert cache.lens.tolist() == [1, 1, 1] and cache.free_count.item() == 39
+    cache.plan(None, 3)
+    cache.release(None)
+    with pytest.raises(RuntimeError, match="plan again"):
+        cache.commit(plan)
+    assert cache.lens.tolist() == [0, 0, 0] and cache.free_count.item() == 42
+    cache.commit(cache.plan(None, 3))
+    assert cache.lens.tolist() == [1, 1, 1]
+
+
 def test_stack_checks_its_attention_layers():
     with pytest.raises(ValueError, match="attn_norm_w"):
         stack.LayerStack([object()], [object()], attn=[object()])
@@ -172,6 +189,36 @@ def test_release_lets_pages_serve_again():
     assert cache.lens.tolist() == [0, 118] and cache.free_count.item() == 0
     assert sorted(cache.table[1, 1:4].tolist()) == first
     assert attention.status() == 0
+
+
+@pytest.mark.gpu
+def test_a_plan_from_before_a_release_is_refused():
+    """Its lengths and free count would undo the release."""
+    cache = attn_layers.PagedKVCache(1, 6, 1, 64, 2, 128, page_size=32)
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    cache.commit(cache.plan(ints([40, 40]), 80))
+    plan = cache.plan(ints([1, 0]), 1)
+    cache.release(ints([0, 1]))
+    with pytest.raises(RuntimeError, match="plan again"):
+        cache.commit(plan)
+    assert cache.lens.tolist() == [40, 0] and cache.free_count.item() == 4
+    plan = cache.plan(ints([1, 90]), 91)
+    cache.commit(plan)
+    assert cache.lens.tolist() == [41, 90] and cache.free_count.item() == 1
+    assert len({*cache.table[0, :2].tolist(), *cache.table[1, :3].tolist()}) == 5
+    cache.commit(plan)  # twice is once
+    assert cache.lens.tolist() == [41, 90] and attention.status() == 0
+
+    # a plan in a graph is made anew by every replay
+    new = ints([0, 1])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan = cache.plan(new, 1)
+    cache.release(ints([1, 0]))
+    graph.replay()
+    cache.commit(plan)
+    assert cache.lens.tolist() == [0, 91] and cache.free_count.item() == 3 and attention.status() == 0
 
 
 def _stack(tmp_path, seed):
