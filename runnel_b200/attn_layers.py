@@ -126,6 +126,10 @@ class GatedAttention(torch.nn.Module):
         plan's last token come out undefined but finite.  ``layer`` indexes the
         cache's layers; ``positions`` (``[axes, T]``) replaces the plan's for images.
         ``record`` (a dict) receives the intermediate tensors, for checking."""
+        with torch.cuda.device_of(x):  # (the products launch on the current device)
+            return self._forward(x, cache, layer, plan, max_q, positions, window, record)
+
+    def _forward(self, x, cache, layer, plan, max_q, positions, window, record):
         T, D, Hq, Hkv = x.shape[0], self.head_dim, self.n_heads, self.n_kv_heads
         y = probes.qmm(self.bits, self.weight, self.scales, self.biases, x, out_f32=False)
         n = Hq * D * (2 if self.gated else 1)

@@ -83,6 +83,10 @@ class LayerStack:
         T, H = x.shape
         if any(a is not None for a in self.attn) and (cache is None or plan is None):
             raise ValueError("attention layers need a cache and a plan")
+        with torch.cuda.device_of(x):  # (blocks and products launch on the current device)
+            return self._forward(x, out, record, cache, plan, max_q, positions)
+
+    def _forward(self, x, out, record, cache, plan, max_q, positions):
         if out is None:
             out = torch.empty_like(x)
         resid_bufs = (torch.empty_like(x), torch.empty_like(x))  # the residual stream, alternating

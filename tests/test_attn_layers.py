@@ -115,6 +115,43 @@ def test_a_release_makes_plans_stale(monkeypatch):
     assert cache.lens.tolist() == [1, 1, 1]
 
 
+def test_layers_run_on_the_device_of_their_tokens(monkeypatch):
+    """The products launch on the current device: the layer and the stack make it that of their tokens."""
+    at, current = [], [0]
+
+    class DeviceOf:
+        def __init__(self, t):
+            self.index = int(t[0, 0])  # (stands in for the tensor's device)
+
+        def __enter__(self):
+            self.was, current[0] = current[0], self.index
+
+        def __exit__(self, *exc):
+            current[0] = self.was
+
+    class Stop(Exception):
+        pass
+
+    def first_call(*a, **k):
+        at.append(current[0])
+        raise Stop
+
+    monkeypatch.setattr(torch.cuda, "device_of", DeviceOf)
+    monkeypatch.setattr(attn_layers.probes, "qmm", first_call)
+    monkeypatch.setattr(stack, "add_rmsnorm", first_call)
+    x = torch.full((1, 512), 3.0)
+    layer = attn_layers.GatedAttention.__new__(attn_layers.GatedAttention)
+    torch.nn.Module.__init__(layer)
+    for n in ("head_dim", "n_heads", "n_kv_heads", "bits", "weight", "scales", "biases", "rotary", "gated"):
+        object.__setattr__(layer, n, 1)
+    s = stack.LayerStack([object()], [object()], attn=[layer], attn_norm_w=[object()])
+    with pytest.raises(Stop):
+        layer.forward(x, None, 0, None)
+    with pytest.raises(Stop):
+        s.forward(x, cache=object(), plan=object())
+    assert at == [3, 3] and current == [0]
+
+
 def test_stack_checks_its_attention_layers():
     with pytest.raises(ValueError, match="attn_norm_w"):
         stack.LayerStack([object()], [object()], attn=[object()])
