@@ -72,21 +72,27 @@ class LayerStack:
                   ctypes.c_float(self.eps), _ptr(resid_out), _ptr(xn), _ptr(y), wp, wn, _stream())
 
     def forward(self, x: torch.Tensor, out: torch.Tensor | None = None, record: list | None = None, cache=None,
-                plan=None, max_q: int | None = None, positions: torch.Tensor | None = None) -> torch.Tensor:
+                plan=None, max_q: int | None = None, positions: torch.Tensor | None = None,
+                window=0) -> torch.Tensor:
         """[T, H] bf16 -> [T, H] bf16.  ``record`` (a list) receives per layer
         (norm input x, block input xn, block output y) copies, for checking.
 
         With attention layers, ``cache`` and ``plan`` are the batch's cache and
         this step's plan (``cache.plan``; T is its ``max_tokens``); attention layer i
         of the stack uses the cache's layer i.  ``max_q``, a bound on a request's
-        rows, and ``positions`` go to the attention layers."""
+        rows, and ``positions`` go to the attention layers, and so does ``window``:
+        a number for all of them (0: none), or one for each attention layer."""
         T, H = x.shape
         if any(a is not None for a in self.attn) and (cache is None or plan is None):
             raise ValueError("attention layers need a cache and a plan")
+        n = sum(a is not None for a in self.attn)
+        windows = [window] * n if isinstance(window, int) else list(window)
+        if len(windows) != n:
+            raise ValueError(f"window must be a number, or one for each of the {n} attention layers")
         with torch.cuda.device_of(x):  # (blocks and products launch on the current device)
-            return self._forward(x, out, record, cache, plan, max_q, positions)
+            return self._forward(x, out, record, cache, plan, max_q, positions, windows)
 
-    def _forward(self, x, out, record, cache, plan, max_q, positions):
+    def _forward(self, x, out, record, cache, plan, max_q, positions, windows):
         if out is None:
             out = torch.empty_like(x)
         resid_bufs = (torch.empty_like(x), torch.empty_like(x))  # the residual stream, alternating
@@ -99,7 +105,7 @@ class LayerStack:
                 if mid is None:
                     mid = torch.empty_like(x)
                 add_rmsnorm(resid, y_prev, self.attn_norm_w[l], mid, xn, self.eps)
-                resid, y_prev = mid, self.attn[l](xn, cache, n_attn, plan, max_q, positions)
+                resid, y_prev = mid, self.attn[l](xn, cache, n_attn, plan, max_q, positions, windows[n_attn])
                 n_attn += 1
             r_out = resid_bufs[l % 2]
             self._layer(bt, resid, y_prev, self.norm_w[l], r_out, xn, y)

@@ -324,6 +324,36 @@ def test_stack_with_attention_steps_and_graph(tmp_path):
 
 
 @pytest.mark.gpu
+def test_stack_hands_windows_to_its_attention_layers(tmp_path):
+    """One window for all of them, or one each: the two layers of a stack against the calls it is made of."""
+    one = _stack(tmp_path, 14)
+    a, an = one.attn[1], one.attn_norm_w[1]
+    s = stack.LayerStack(one.layers, one.norm_w, ws=one.ws, attn=[a, a], attn_norm_w=[an, an])
+    g = torch.Generator(device=DEV).manual_seed(15)
+    x = torch.randn(90, 2048, generator=g, device=DEV).to(torch.bfloat16)
+    new = torch.tensor([60, 0, 30], dtype=torch.int32, device=DEV)
+    got = {}
+    for window in (0, 7, (0, 7), (7, 0)):
+        cache = _cache(2, 2, 128, 3)
+        plan = cache.plan(new, 90)
+        got[window] = s.forward(x, cache=cache, plan=plan, window=window)
+        each = (window, window) if isinstance(window, int) else window
+        r, xn, y = torch.empty_like(x), torch.empty_like(x), None
+        for i, w in enumerate(each):
+            stack.add_rmsnorm(r if i else x, y, an, r, xn)
+            y = a(xn, cache, i, plan, window=w)
+            stack.add_rmsnorm(r, y, s.norm_w[i], r, xn)
+            y = ops.moe_block(s.layers[i], xn)
+        stack.add_rmsnorm(r, y, s.norm_w[1], r, xn)
+        assert torch.equal(r, got[window])
+    assert not any(torch.equal(got[u], got[v]) for u, v in ((0, 7), ((0, 7), (7, 0)), (0, (0, 7)), (7, (7, 0))))
+    for window in ((), (1,), (1, 2, 3)):
+        with pytest.raises(ValueError, match="window"):
+            s.forward(x, cache=cache, plan=plan, window=window)
+    assert attention.status() == 0
+
+
+@pytest.mark.gpu
 def test_stack_refuses_attention_without_a_cache(tmp_path):
     s = _stack(tmp_path, 13)
     with pytest.raises(ValueError, match="cache and a plan"):
