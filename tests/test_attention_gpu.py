@@ -731,6 +731,34 @@ def test_status_reads_lose_no_bit_of_another_stream():
         assert seen | attention.status() == _lib.STATUS_NO_PAGES
 
 
+@pytest.mark.parametrize("Hq,Hkv,D,lens,rows", [
+    (16, 2, 256, [2000, 300], [200, 90]),  # many rows, whole tiles
+    (16, 2, 256, [5000], [40]), (12, 1, 128, [9000, 300], [7, 7]),  # split and joined
+    (32, 8, 128, [700, 90, 3000], [300, 1, 4]),  # both kernels
+])
+def test_many_rows_on_several_streams(Hq, Hkv, D, lens, rows):
+    """Overlapping calls of the many-row kernel, and a status read beside them, as if each were alone."""
+    g = _gen(sum(lens) + D)
+    kc, vc, table = _cache_of(g, BF16, lens, Hkv, D, 64)
+    sl, cu = _i(lens), _i([0, *itertools.accumulate(rows)])
+    qs = [_rand(g, BF16, sum(rows), Hq, D) for _ in range(4)]
+    call = lambda q: attention.paged_attention(q, kc, vc, table, sl, cu_q=cu, max_q=max(rows), return_lse=True)  # noqa: E731
+    want = [call(q) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    got = [[] for _ in qs]
+    for n in range(20):
+        for i, (q, s) in enumerate(zip(qs, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(call(q))
+        if n % 7 == 3:
+            assert attention.status() == 0
+    torch.cuda.synchronize()
+    for w, outs in zip(want, got):
+        assert all(torch.equal(o, w[0]) and torch.equal(e, w[1]) for o, e in outs)
+    assert attention.status() == 0
+
+
 def test_refusals_on_the_device():
     g = _gen(15)
     kc, vc, table = _cache_of(g, BF16, [20, 20], 2, 64, 16)
