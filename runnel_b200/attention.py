@@ -16,8 +16,12 @@ A layer's cache is two tensors ``[num_pages, n_kv_heads, page_size, head_dim]``
 (bf16 or fp16; page and head strides are free).  Lengths, tables, slots and
 positions are int32 CUDA tensors and stay on the device.  Calls are
 asynchronous on the current stream of their tensors' device and can be captured
-in a CUDA graph; each takes its scratch from torch's allocator unless it is
-given one.  Nothing falls back to another implementation.
+in a CUDA graph; each takes its scratch from torch's allocator.  Nothing falls
+back to another implementation.
+
+What goes wrong on the device (plans that do not fit, ids and lengths out of
+range, a wait that gave up) shows in :func:`status` alone, so a server reads it every
+so many steps.
 """
 from __future__ import annotations
 
@@ -156,6 +160,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     behind ``cu_q[-1]`` are left as they were.  ``out`` may be ``q`` if that is contiguous,
     but not share memory with it otherwise, nor with ``gate``.  ``max_q``, a bound on the rows of one
     request, picks the kernels and is worth giving.
+
+    Device waits are bounded: after one that gave up (a second), :func:`status` has
+    ``STATUS_TIMEOUT``, the outputs since are void, and until it is read the rows of
+    many-row requests are left unwritten, on every stream of the device (without
+    ``out``, they are memory as it was allocated).
     """
     return (_calls or _native()).paged_attention(q, k_cache, v_cache, table, seq_lens, cu_q, max_q, scale, window, gate, out,
                                                  return_lse)

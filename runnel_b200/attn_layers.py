@@ -9,9 +9,13 @@ projections, normed and rotated heads, causal attention, output gate).
     plan = cache.plan(new_lens, max_tokens)       # pages, slots, positions of the step's tokens
     out = stack.forward(x, cache=cache, plan=plan, max_q=longest)   # x [max_tokens, H], requests in order
     cache.commit(plan)
+    cache.release(finished)                       # requests that are done, before the next plan
 
 Everything that varies from step to step (lengths, pages, positions) is on the
-device, so a step of fixed ``max_tokens`` can be captured in a CUDA graph.
+device, so a step of fixed ``max_tokens`` can be captured in a CUDA graph.  Neither
+the cache nor the layers read :func:`runnel_b200.attention.status`, which waits for the
+device: the caller does, every so many steps (a plan that did not fit, a page id out
+of range, and ``STATUS_TIMEOUT``, after which outputs are void until it is read).
 """
 from __future__ import annotations
 

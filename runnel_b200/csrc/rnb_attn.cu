@@ -680,7 +680,6 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
     for (int w = 1; w < kWays; ++w) {
       const float4 v = acc_s[w][col];
       acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
-      ls += lred[w];
     }
     ls = lred[0];
 #pragma unroll

@@ -14,12 +14,15 @@
 // * The maximum is lazy: m only moves when a row's maximum exceeds it by more
 //   than 8 (P stays below 2^8, in range of both types), so O is hardly ever
 //   rescaled after the first blocks.
-// * Slots of S keep the tensor cores and the softmax apart: S of later blocks is
-//   computed before P of this one is done.  With head_dim <= 128 there are two row
-//   tiles with a softmax warpgroup and two slots of 64 positions each (one slot of 128
-//   each made a warpgroup wait for its own two products every block: 3900
-//   cycles a 128 positions); with 256, where one O fills half the tensor memory, two
-//   slots of 128 positions of one tile.
+// * Two slots of S, a block of 128 positions each, keep the tensor cores and the
+//   softmax apart.  With head_dim <= 128 there are two row tiles with a softmax
+//   warpgroup and one slot each: one tile's products run under the other's softmax,
+//   but a tile's own chain softmax, P V, next Q K is in series, since P lies in the
+//   slot (3900 cycles a block, of which the products take 2048).  Two slots of 64 a
+//   tile were slower: products of N = 64 read shared memory at its limit (8192 rows at
+//   128: 626 instead of 534 us).  With 256, where one O fills half the tensor memory,
+//   one tile has both slots, and S of a block is computed before P of the one before
+//   it is done.
 // * Keys and values come by TMA page by page into a ring of 128-byte-swizzled
 //   units, K as the K-major and V as the MN-major operand, both as they lie in the
 //   cache.  Pages behind the request's end (and ids out of range) are fetched at
@@ -591,8 +594,9 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
         m = to;
         l *= f;
         if (i > 0) {
-          // the product before this one has to be in O (the one before that is:
-          // S of this block was issued behind it)
+          // the product before this one has to be in O (with two slots a tile the one
+          // before that is, since S of this block was issued behind it; with one
+          // slot S was issued behind this very product)
           alive = wait_on(&bars.o_done[wg], (i - 1) & 1);
           if (!alive) break;
           tc_fence_after();
@@ -635,8 +639,8 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
       l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
     }
     // ---- O / l
-    // (o_done would not do: the last two products may both be under way, and a
-    // parity only tells neighbouring phases apart)
+    // (o_done would not do: with two slots a tile the last two products may both be
+    // under way, and a parity only tells neighbouring phases apart)
     if (alive && nblk > 0) alive = wait_on(&bars.o_last[wg], 0);
     tc_fence_after();
     if (parts > 1) {
