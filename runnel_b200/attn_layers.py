@@ -109,6 +109,16 @@ class GatedAttention(torch.nn.Module):
         for p in (q_proj, k_proj, v_proj, o_proj):
             if p.group_size != 64 or p.mode != "affine" or p.get("biases") is None or "bias" in p:
                 raise ValueError("projections must be affine-quantized in groups of 64, without module biases")
+        # the products read as many scales and biases as the codes' shape says
+        for name, p in (("q_proj", q_proj), ("k_proj", k_proj), ("v_proj", v_proj), ("o_proj", o_proj)):
+            groups = (p.weight.shape[0], p.weight.shape[1] * 32 // p.bits // 64)
+            if p.weight.dtype not in (torch.uint32, torch.int32) or any(
+                    t.dtype != torch.bfloat16 or tuple(t.shape) != groups for t in (p.scales, p.biases)):
+                raise ValueError(f"{name} must have 32-bit codes, and bf16 scales and biases of shape {groups}")
+        self.hidden = q_proj.weight.shape[1] * 32 // q_proj.bits
+        if o_proj.weight.shape[0] != self.hidden or any(p.weight.shape[1] != q_proj.weight.shape[1]
+                                                        for p in (k_proj, v_proj)):
+            raise ValueError(f"projections must all fit the hidden size of q_proj, {self.hidden}")
         self.head_dim, self.rotary, self.gated, self.eps = head_dim, rotary, gated, eps
         self.bits, self.o_bits = q_proj.bits, o_proj.bits
         self.n_heads = o_proj.weight.shape[-1] * 32 // o_proj.bits // head_dim
@@ -116,6 +126,12 @@ class GatedAttention(torch.nn.Module):
         q_rows = self.n_heads * head_dim * (2 if gated else 1)
         if q_proj.weight.shape[0] != q_rows or v_proj.weight.shape[0] != k_proj.weight.shape[0]:
             raise ValueError(f"q_proj must have {q_rows} rows, k_proj and v_proj as many as each other")
+        if k_proj.weight.shape[0] % head_dim or self.n_kv_heads == 0 or self.n_heads % self.n_kv_heads:
+            raise ValueError(f"k_proj must have the rows of heads of {head_dim}, of which the {self.n_heads} query heads "
+                             "are a multiple")
+        for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+            if w is not None and (w.dtype != torch.bfloat16 or tuple(w.shape) != (head_dim,)):
+                raise ValueError(f"{name} must be bf16 [{head_dim}]")
         for n in ("weight", "scales", "biases"):
             self.register_buffer(n, _cat([getattr(m, n) for m in (q_proj, k_proj, v_proj)], 0))
         self.o_proj = o_proj
@@ -130,6 +146,8 @@ class GatedAttention(torch.nn.Module):
         plan's last token come out undefined but finite.  ``layer`` indexes the
         cache's layers; ``positions`` (``[axes, T]``) replaces the plan's for images.
         ``record`` (a dict) receives the intermediate tensors, for checking."""
+        if x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[1] != self.hidden:
+            raise ValueError(f"x must be bf16 [tokens, {self.hidden}], not {x.dtype} {tuple(x.shape)}")
         with torch.cuda.device_of(x):  # (the products launch on the current device)
             return self._forward(x, cache, layer, plan, max_q, positions, window, record)
 

@@ -85,6 +85,9 @@ class LayerStack:
         T, H = x.shape
         if any(a is not None for a in self.attn) and (cache is None or plan is None):
             raise ValueError("attention layers need a cache and a plan")
+        for w in self.attn_norm_w:
+            if w is not None and (w.dtype != torch.bfloat16 or w.shape != (H,)):
+                raise ValueError(f"attn_norm_w must be bf16 [{H}]")
         n = sum(a is not None for a in self.attn)
         windows = [window] * n if isinstance(window, int) else list(window)
         if len(windows) != n:

@@ -115,6 +115,65 @@ def test_a_release_makes_plans_stale(monkeypatch):
     assert cache.lens.tolist() == [1, 1, 1]
 
 
+def _cpu_linears(rng, H=512, Hq=8, Hkv=2, D=64):
+    def linear(rows, K):
+        w, s, b = (torch.from_numpy(a.view(np.int32 if a.dtype == np.uint32 else np.int16))
+                   for a in _linear_arrays(rng, rows, K, 4))
+        return [w.view(torch.uint32), s.view(torch.bfloat16), b.view(torch.bfloat16)]
+    return {"q_proj": linear(2 * Hq * D, H), "k_proj": linear(Hkv * D, H), "v_proj": linear(Hkv * D, H),
+            "o_proj": linear(H, Hq * D)}
+
+
+def test_attention_layer_refuses_shapes_that_do_not_fit():
+    """The products read what the codes' shape says: scales, biases and sizes have to agree with it."""
+    def layer(lin, D=64, norm=None):
+        return attn_layers.GatedAttention(**{n: QuantizedLinear(*t) for n, t in lin.items()}, q_norm=norm, k_norm=None,
+                                          head_dim=D, rotary=attn_layers.RotarySpec(32))
+
+    new = lambda: _cpu_linears(np.random.default_rng(6))  # noqa: E731
+    assert layer(new()).n_heads == 8
+    for proj in ("q_proj", "k_proj", "v_proj", "o_proj"):
+        for part, cut in ((1, lambda t: t[:-1]), (2, lambda t: t[:-1]), (1, lambda t: t[:, :-1]), (2, lambda t: t[:, :-1]),
+                          (1, lambda t: t.half()), (2, lambda t: t.float()), (0, lambda t: t.view(torch.int32).long())):
+            lin = new()
+            lin[proj][part] = cut(lin[proj][part])
+            with pytest.raises(ValueError, match=proj):
+                layer(lin)
+    lin = new()
+    lin["v_proj"] = [t[:, :t.shape[1] // 2] for t in lin["v_proj"]]  # another hidden size
+    with pytest.raises(ValueError, match="hidden"):
+        layer(lin)
+    lin = new()
+    lin["o_proj"] = [t[:256] for t in lin["o_proj"]]
+    with pytest.raises(ValueError, match="hidden"):
+        layer(lin)
+    lin = new()
+    for proj in ("k_proj", "v_proj"):
+        lin[proj] = [t[:100] for t in lin[proj]]  # not whole heads
+    with pytest.raises(ValueError, match="heads"):
+        layer(lin)
+    lin = _cpu_linears(np.random.default_rng(7), Hkv=3)
+    with pytest.raises(ValueError, match="heads"):
+        layer(lin)
+    for norm in (torch.ones(63, dtype=torch.bfloat16), torch.ones(64), torch.ones(1, 64, dtype=torch.bfloat16)):
+        with pytest.raises(ValueError, match="q_norm"):
+            layer(new(), norm=norm)
+
+
+def test_attention_layers_refuse_tokens_that_are_not_bf16_rows():
+    a = attn_layers.GatedAttention(**{n: QuantizedLinear(*t) for n, t in _cpu_linears(np.random.default_rng(8)).items()},
+                                   q_norm=None, k_norm=None, head_dim=64, rotary=attn_layers.RotarySpec(32))
+    for x in (torch.zeros(3, 512), torch.zeros(3, 512, dtype=torch.float16), torch.zeros(3, 256, dtype=torch.bfloat16),
+              torch.zeros(1, 3, 512, dtype=torch.bfloat16), torch.zeros(512, dtype=torch.bfloat16)):
+        with pytest.raises(ValueError, match="bf16"):
+            a(x, None, 0, None)
+    x = torch.zeros(3, 512, dtype=torch.bfloat16)
+    for norm in (torch.ones(511, dtype=torch.bfloat16), torch.ones(512)):
+        s = stack.LayerStack([object()], [object()], attn=[a], attn_norm_w=[norm])
+        with pytest.raises(ValueError, match="attn_norm_w"):
+            s.forward(x, cache=object(), plan=object())
+
+
 def test_layers_run_on_the_device_of_their_tokens(monkeypatch):
     """The products launch on the current device: the layer and the stack make it that of their tokens."""
     at, current = [], [0]
@@ -139,12 +198,10 @@ def test_layers_run_on_the_device_of_their_tokens(monkeypatch):
     monkeypatch.setattr(torch.cuda, "device_of", DeviceOf)
     monkeypatch.setattr(attn_layers.probes, "qmm", first_call)
     monkeypatch.setattr(stack, "add_rmsnorm", first_call)
-    x = torch.full((1, 512), 3.0)
-    layer = attn_layers.GatedAttention.__new__(attn_layers.GatedAttention)
-    torch.nn.Module.__init__(layer)
-    for n in ("head_dim", "n_heads", "n_kv_heads", "bits", "weight", "scales", "biases", "rotary", "gated"):
-        object.__setattr__(layer, n, 1)
-    s = stack.LayerStack([object()], [object()], attn=[layer], attn_norm_w=[object()])
+    x = torch.full((1, 512), 3.0, dtype=torch.bfloat16)
+    layer = attn_layers.GatedAttention(**{n: QuantizedLinear(*t) for n, t in _cpu_linears(np.random.default_rng(9)).items()},
+                                       q_norm=None, k_norm=None, head_dim=64, rotary=attn_layers.RotarySpec(32))
+    s = stack.LayerStack([object()], [object()], attn=[layer], attn_norm_w=[torch.ones(512, dtype=torch.bfloat16)])
     with pytest.raises(Stop):
         layer.forward(x, None, 0, None)
     with pytest.raises(Stop):
