@@ -148,6 +148,8 @@ class GatedAttention(torch.nn.Module):
         ``record`` (a dict) receives the intermediate tensors, for checking."""
         if x.dtype != torch.bfloat16 or x.dim() != 2 or x.shape[1] != self.hidden:
             raise ValueError(f"x must be bf16 [tokens, {self.hidden}], not {x.dtype} {tuple(x.shape)}")
+        if x.shape[0] == 0:
+            return torch.empty_like(x)
         with torch.cuda.device_of(x):  # (the products launch on the current device)
             return self._forward(x, cache, layer, plan, max_q, positions, window, record)
 

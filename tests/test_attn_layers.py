@@ -265,6 +265,17 @@ def test_layer_stages_against_64_bits(tmp_path, gated, sections):
 
 
 @pytest.mark.gpu
+def test_layer_of_no_tokens(tmp_path):
+    st = _write(tmp_path, np.random.default_rng(20), 512, 8, 2, 64)
+    layer, _ = checkpoint.load_attention(st, 3, attn_layers.RotarySpec(rot=32), device=DEV)
+    cache = _cache(1, 2, 64, 3)
+    plan = cache.plan(torch.zeros(3, dtype=torch.int32, device=DEV), 0)
+    assert layer(torch.zeros(0, 512, dtype=torch.bfloat16, device=DEV), cache, 0, plan).shape == (0, 512)
+    cache.commit(plan)
+    assert cache.lens.tolist() == [0, 0, 0] and attention.status() == 0
+
+
+@pytest.mark.gpu
 def test_release_lets_pages_serve_again():
     cache = attn_layers.PagedKVCache(1, 4, 1, 64, 2, 128, page_size=32)
     new = torch.tensor([100, 28], dtype=torch.int32, device=DEV)
