@@ -152,29 +152,31 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_plan(const PlanArgs a) {
     for (int i = 0; i < kAhead; ++i)
       if (tid + i * kPlanThreads < need) top = max(top, ahead[i]);
 #pragma unroll 4
-    for (int n = tid + kAhead * kPlanThreads; n < need; n += kPlanThreads)
-      top = max(top, static_cast<uint32_t>(next_free[-n]));
+    for (uint32_t n = tid + kAhead * kPlanThreads; n < static_cast<uint32_t>(need); n += kPlanThreads)
+      top = max(top, static_cast<uint32_t>(next_free[-static_cast<int64_t>(n)]));
   }
   const bool strange = __syncthreads_or(top >= static_cast<uint32_t>(a.num_pages));
   ok = ok && !strange;
   const int tokens = ok ? static_cast<int>(tot[0]) : 0, pages = ok ? static_cast<int>(tot[1]) : 0;
 
-  const int stride = gridDim.x * kPlanThreads, at = blockIdx.x * kPlanThreads + tid;
+  // (unsigned: a step past the last of almost 2^31 rows or pages stays a number)
+  const uint32_t stride = gridDim.x * kPlanThreads, at = blockIdx.x * kPlanThreads + tid;
   if (at == 0) {
     a.cu[a.B] = tokens;
     *a.free_out = fc - pages;
     if (!ok) atomicOr(&g_kv_status, RNB_STATUS_NO_PAGES | (strange ? RNB_STATUS_BAD_INDEX : 0));
   }
-  for (int b = at; b < a.B; b += stride) {
+  for (uint32_t b = at; b < static_cast<uint32_t>(a.B); b += stride) {
     a.cu[b] = ok ? cu[b] : 0;
     a.seq[b] = a.ctx[b] + (ok ? a.fresh[b] : 0);
   }
-  for (int n = at; n < pages; n += stride) {
-    const int b = find_request(base, a.B, n);
+  for (uint32_t i = at; i < static_cast<uint32_t>(pages); i += stride) {
+    const int n = static_cast<int>(i), b = find_request(base, a.B, n);
     const int held = static_cast<int>((static_cast<int64_t>(a.ctx[b]) + P - 1) >> a.log2p);
     a.table[static_cast<int64_t>(b) * a.W + held + (n - base[b])] = a.free_pages[fc - 1 - n];
   }
-  for (int t = at; t < a.max_tokens; t += stride) {
+  for (uint32_t i = at; i < static_cast<uint32_t>(a.max_tokens); i += stride) {
+    const int t = static_cast<int>(i);
     int pos = 0, slot = -1;
     if (t < tokens) {
       const int b = find_request(cu, a.B, t);
@@ -255,8 +257,9 @@ __global__ void __launch_bounds__(kPlanThreads) k_kv_release(const ReleaseArgs a
   // entries that are no pages need no room: where not all entries fit, the pages are counted first
   for (int pass = held <= a.free_capacity - fc ? 1 : 0; pass < 2 && ok; ++pass) {
     pages = 0;
-    for (int n0 = 0; n0 < held; n0 += kPlanThreads) {
-      const int id = n0 + tid < held ? entry(n0 + tid) : -1;
+    for (uint32_t n0 = 0; n0 < static_cast<uint32_t>(held); n0 += kPlanThreads) {
+      const uint32_t n = n0 + tid;
+      const int id = n < static_cast<uint32_t>(held) ? entry(static_cast<int>(n)) : -1;
       const bool page = id >= 0 && id < a.num_pages;
       strange = strange || id >= a.num_pages;
       int all;
@@ -330,7 +333,7 @@ int rnb_kv_plan(int B, int table_cols, int page_size, int num_pages, int max_tok
   // sums over the requests, so more CTAs would only repeat them again
   const int work = max_tokens > B ? max_tokens : B;
   const int sms = dev_info().sms;
-  int grid = (work + kPlanThreads - 1) / kPlanThreads;
+  int grid = work / kPlanThreads + (work % kPlanThreads ? 1 : 0);
   grid = grid < 1 ? 1 : grid > sms ? sms : grid;
   const PlanArgs a{B, table_cols, log2_of(page_size), num_pages, max_tokens, free_capacity, table, ctx_lens, new_lens,
                    free_pages, free_count, seq_lens, cu_q, positions, slots, free_count_out};

@@ -166,6 +166,20 @@ def test_plan_that_would_take_a_bad_id_is_void(need, at, bad):
     assert attention.status() == 0
 
 
+def test_plan_of_almost_2_to_31_rows():
+    """The rows behind the last request are filled to the end, and nothing else is."""
+    n = 2 ** 31 - 1
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 17 GB for positions and slots")
+    t = torch.zeros(2, 3, dtype=torch.int32, device=DEV)
+    p = attention.kv_plan(t, _i([0, 5]), _i([17, 1]), _i([4, 3, 2]), _i([3]), page_size=16, num_pages=8, max_tokens=n)
+    assert p.slots[:20].tolist() == [*range(32, 48), 48, 5, -1, -1] and p.slots.numel() == n
+    assert p.positions[:20].tolist() == [*range(17), 5, 0, 0]
+    for i in range(18, n, 1 << 28):
+        assert (p.slots[i:i + (1 << 28)] == -1).all() and not p.positions[i:i + (1 << 28)].any()
+    assert p.cu_q.tolist() == [0, 17, 18] and p.free_count.item() == 1 and attention.status() == 0
+
+
 def test_plan_of_no_requests():
     e = torch.zeros(0, dtype=torch.int32, device=DEV)
     p = attention.kv_plan(e.view(0, 3), e, e, _i([4, 5]), _i([2]), page_size=16, num_pages=6, max_tokens=3)
