@@ -495,8 +495,9 @@ RNB_API int rnb_rope_append(const rnb_rope_desc* d, const void* q, const void* k
  * (0: unknown) bounds the rows of a request and only picks the kernels.  The
  * workspace needs no initial state; calls that may overlap need one each.  Results do not depend
  * on timing: equal inputs give equal bits.  A device wait inside the many-row
- * kernel that gives up after a second sets RNB_STATUS_TIMEOUT: results are void
- * then, and until the status is read many-row requests are left out. */
+ * kernel that gives up after a second sets RNB_STATUS_TIMEOUT: that call's
+ * results are void then, and the rest of its many-row requests are left out (in a
+ * captured call's replays too, until the status is read). */
 typedef struct rnb_attn_desc {
   int32_t B;
   int32_t T;          /* rows of q and out */

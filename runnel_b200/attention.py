@@ -162,9 +162,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     request, picks the kernels and is worth giving.
 
     Device waits are bounded: after one that gave up (a second), :func:`status` has
-    ``STATUS_TIMEOUT``, the outputs since are void, and until it is read the rows of
-    many-row requests are left unwritten, on every stream of the device (without
-    ``out``, they are memory as it was allocated).
+    ``STATUS_TIMEOUT`` and that call's outputs are void: the rest of its many-row requests
+    are left unwritten (without ``out``, memory as it was allocated), and so they are
+    where a graph replays the call, until the status is read.
     """
     return (_calls or _native()).paged_attention(q, k_cache, v_cache, table, seq_lens, cu_q, max_q, scale, window, gate, out,
                                                  return_lse)

@@ -15,7 +15,8 @@ Everything that varies from step to step (lengths, pages, positions) is on the
 device, so a step of fixed ``max_tokens`` can be captured in a CUDA graph.  Neither
 the cache nor the layers read :func:`runnel_b200.attention.status`, which waits for the
 device: the caller does, every so many steps (a plan that did not fit, a page id out
-of range, and ``STATUS_TIMEOUT``, after which outputs are void until it is read).
+of range, and ``STATUS_TIMEOUT``: a call's outputs are void, a captured one's until it is
+read).
 """
 from __future__ import annotations
 

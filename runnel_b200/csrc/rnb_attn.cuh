@@ -22,6 +22,7 @@ struct AttnArgs {
   int direct;    // few-row kernel: whole tiles by number (one row a request)
   int split;     // many-row kernel: CTAs over which the tiles' positions are split (0: not)
   int few_rows;  // requests with rows * group below this are the few-row kernel's
+  uint32_t call;  // many-row kernel: the call's number, not 0
 };
 
 // The many-row kernel (rnb_attn_prompt.cu): TMA maps of the call's tensors, and

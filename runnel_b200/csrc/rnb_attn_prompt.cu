@@ -40,6 +40,7 @@
 #include <limits.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <string>
 
 #include "rnb_attn.cuh"
@@ -49,6 +50,10 @@ namespace rnb {
 namespace {
 
 __device__ uint32_t g_prompt_status;
+// The call whose wait gave up last (0: none).  A grid of CTAs that each wait their
+// second would hold the device for minutes, so the rest of that call does nothing;
+// other calls, on whatever stream, go on.
+__device__ uint32_t g_gave_up;
 
 constexpr uint64_t kWaitNs = 1000000000ull;
 
@@ -259,9 +264,7 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
       // (of several requests the few-row kernel tells)
       if (a.B == 1 && blockIdx.x == 0 && (a.cu[0] < 0 || a.cu[1] < a.cu[0] || a.cu[1] > a.T))
         atomicOr(&g_prompt_status, RNB_STATUS_BAD_INDEX);
-      // after a wait that gave up, until the status is read: a grid of CTAs that
-      // each wait their second would hold the device for minutes
-      gave_up = *const_cast<volatile uint32_t*>(&g_prompt_status) & RNB_STATUS_TIMEOUT;
+      gave_up = *const_cast<volatile uint32_t*>(&g_gave_up) == a.call;
     }
     const int per = (a.B + C::kThreads - 1) / C::kThreads;
     const int lo = min(tid * per, a.B), hi = min(lo + per, a.B);
@@ -723,7 +726,10 @@ __global__ void __launch_bounds__(Cfg<D>::kThreads, 1)
       }
     }
   }
-  if (!alive && lane == 0) atomicOr(&g_prompt_status, RNB_STATUS_TIMEOUT);
+  if (!alive && lane == 0) {
+    atomicExch(&g_gave_up, a.call);
+    atomicOr(&g_prompt_status, RNB_STATUS_TIMEOUT);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -813,6 +819,7 @@ bool encode_rows(CUtensorMap* m, const AttnArgs& a, const void* base, int D, int
 }  // namespace
 
 cudaError_t prompt_status_word(uint32_t** p) { return status_word(g_prompt_status, p); }
+cudaError_t prompt_gave_up_word(uint32_t** p) { return status_word(g_gave_up, p); }
 
 bool prepare_prompt(const AttnArgs& a, const rnb_kv_cache* c, PromptMaps* p) {
   if (a.group > 128) return false;
@@ -846,7 +853,11 @@ int plan_split(AttnArgs* a, int D, int sms, size_t* bytes) {
   return a->split;
 }
 
-int run_prompt(const AttnArgs& a, const rnb_kv_cache* c, const PromptMaps& p, cudaStream_t st) {
+int run_prompt(const AttnArgs& args, const rnb_kv_cache* c, const PromptMaps& p, cudaStream_t st) {
+  static std::atomic<uint32_t> calls{0};
+  AttnArgs a = args;
+  do a.call = ++calls;
+  while (a.call == 0);
   const int D = c->head_dim;
   if (c->dtype == RNB_DTYPE_BF16) {
     if (D == 64) return launch_prompt<__nv_bfloat16, 64>(a, p, st);

@@ -38,11 +38,13 @@ __device__ uint32_t g_status_taken;
 
 struct StatusWords {
   uint32_t* word[4];
+  uint32_t* gave_up;
 };
 
 __global__ void k_take_status(const StatusWords s) {
   uint32_t bits = 0;
   for (uint32_t* w : s.word) bits |= atomicExch(w, 0u);
+  if (bits & RNB_STATUS_TIMEOUT) atomicExch(s.gave_up, 0u);  // (a captured call may run again)
   g_status_taken = bits;
 }
 
@@ -381,6 +383,7 @@ int rnb_kv_status(uint32_t* status, void* stream) {
   if (e == cudaSuccess) e = rope_status_word(&words.word[1]);
   if (e == cudaSuccess) e = attn_status_word(&words.word[2]);
   if (e == cudaSuccess) e = prompt_status_word(&words.word[3]);
+  if (e == cudaSuccess) e = prompt_gave_up_word(&words.gave_up);
   if (e == cudaSuccess) {
     k_take_status<<<1, 1, 0, st>>>(words);
     e = cudaGetLastError();

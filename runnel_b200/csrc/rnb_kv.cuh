@@ -92,6 +92,8 @@ __device__ __forceinline__ void after_previous() {
 cudaError_t rope_status_word(uint32_t** p);
 cudaError_t attn_status_word(uint32_t** p);
 cudaError_t prompt_status_word(uint32_t** p);
+// The many-row kernel's word for the call that gave up, which a status read clears.
+cudaError_t prompt_gave_up_word(uint32_t** p);
 
 template <typename Sym>
 inline cudaError_t status_word(Sym& word, uint32_t** p) {

@@ -81,7 +81,9 @@ class LayerStack:
         this step's plan (``cache.plan``; T is its ``max_tokens``); attention layer i
         of the stack uses the cache's layer i.  ``max_q``, a bound on a request's
         rows, and ``positions`` go to the attention layers, and so does ``window``:
-        a number for all of them (0: none), or one for each attention layer."""
+        a number for all of them (0: none), or one for each attention layer.  What went
+        wrong on the device is in :func:`runnel_b200.attention.status` alone, which the
+        caller reads every so many steps."""
         T, H = x.shape
         if any(a is not None for a in self.attn) and (cache is None or plan is None):
             raise ValueError("attention layers need a cache and a plan")
