@@ -11,10 +11,11 @@
 // here (2048 requests, 64 Ki rows) moves 0.5 MB, under 0.1 us of HBM time, so
 // the launch and one trip of dependent loads bound it.  Hence one launch and
 // no grid-wide exchange: every CTA computes both sums over all requests by
-// itself (shared memory, 8 bytes a request), then takes its share of the token
-// rows and of the new pages and finds each one's request by binary search.  A
-// row in a new page takes the id from the free list, not from the table entry
-// that another CTA may be writing.
+// itself (shared memory, 8 bytes a request) and looks at all ids that the step
+// takes, so that all agree on whether the plan is void, then takes its share of
+// the token rows and of the new pages and finds each one's request by binary
+// search.  A row in a new page takes the id from the free list, not from the table
+// entry that another CTA may be writing.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
